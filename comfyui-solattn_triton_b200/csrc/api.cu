@@ -166,9 +166,9 @@ EncodeTiledFn encode_fn() {
 }
 
 // 4-D map over a BTHD-like tensor: dims {D, H, rows, B}, byte strides {head, row, batch},
-// box {64 bf16 (or 128 int8) = 128 bytes, 1, box_rows, 1}, 128-byte swizzle, OOB = zeros.
+// box {64 bf16 (or 128 int8) = 128 bytes, box_heads, box_rows, 1}, 128-byte swizzle, OOB = zeros.
 int32_t make_map(CUtensorMap* m, const void* ptr, bool int8, int64_t D, int64_t H, int64_t rows, int64_t B,
-                 int64_t s_h, int64_t s_row, int64_t s_b, int box_rows, const char* name) {
+                 int64_t s_h, int64_t s_row, int64_t s_b, int box_rows, const char* name, int box_heads = 1) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(SOLB200_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const int64_t esz = int8 ? 1 : 2;
@@ -179,7 +179,7 @@ int32_t make_map(CUtensorMap* m, const void* ptr, bool int8, int64_t D, int64_t 
   // 64-wide head are 64 bytes and use the 64-byte swizzle.
   const cuuint32_t inner = int8 ? (cuuint32_t)(D < 128 ? D : 128) : 64;
   const CUtensorMapSwizzle swz = inner * esz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-  cuuint32_t box[4] = {inner, 1, (cuuint32_t)box_rows, 1};
+  cuuint32_t box[4] = {inner, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, int8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                    const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -674,6 +674,18 @@ namespace solb200 {
 int32_t set_last_error(int32_t code, const std::string& msg) { return fail(code, msg); }
 
 int32_t set_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+int32_t check_sm100() { return check_device(); }
+
+uint64_t current_wait_ns() { return g_debug_wait.wait_ns; }
+
+int32_t bthd_map(CUtensorMap* m, const void* ptr, int64_t D, int64_t H, int64_t rows, int64_t B,
+                 const int64_t* strides, int box_heads, int box_rows, const char* name) {
+  // a dimension of one element may come with any stride: give the map a valid one
+  const int64_t s_h = H == 1 ? D : strides[2];
+  const int64_t s_row = rows == 1 ? H * s_h : strides[1];
+  return make_map(m, ptr, false, D, H, rows, B, s_h, s_row, strides[0], box_rows, name, box_heads);
+}
 
 int32_t plan_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t D, int32_t block, int32_t int8,
                              int64_t* bytes) {

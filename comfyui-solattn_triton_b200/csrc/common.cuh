@@ -348,6 +348,20 @@ __device__ __forceinline__ void named_bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
+// The same barrier with a vote: whether `pred` holds for every participating thread.
+__device__ __forceinline__ bool named_bar_all(int id, int count, bool pred) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(all)
+      : "r"(id), "r"(count), "r"((uint32_t)pred)
+      : "memory");
+  return all != 0;
+}
+
 // Per-warpgroup register budgets (executed by all four warps of a warpgroup together).
 // The increases draw on what the decreases release: the block's launch total (threads x
 // registers per thread at launch) must cover the sum of the new budgets.

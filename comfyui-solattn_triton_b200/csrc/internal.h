@@ -5,6 +5,7 @@
 
 #include <string>
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace solb200 {
@@ -12,6 +13,17 @@ namespace solb200 {
 // Record the calling thread's last-error text and return `code`.
 int32_t set_last_error(int32_t code, const std::string& msg);
 int32_t set_cuda_error(cudaError_t e, const char* what);
+
+// SOLB200_OK when the current device is an sm_100.
+int32_t check_sm100();
+
+// The pipeline wait limit of the calling thread (solb200_debug_set_wait).
+uint64_t current_wait_ns();
+
+// Tensor map of a bf16 [B, rows, H, D] tensor (element strides {batch, row, head}) for boxes of
+// 64 channels x box_heads x box_rows, 128-byte swizzle, zeros outside the tensor.
+int32_t bthd_map(CUtensorMap* m, const void* ptr, int64_t D, int64_t H, int64_t rows, int64_t B,
+                 const int64_t* strides, int box_heads, int box_rows, const char* name);
 
 // Workspace bytes of one attention call with this geometry (solb200_workspace_bytes).
 int32_t plan_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t D, int32_t block, int32_t int8,

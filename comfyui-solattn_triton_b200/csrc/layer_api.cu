@@ -1,0 +1,332 @@
+// Host side of the C ABI's layer operators (include/solb200.h): head norms with the position
+// rotation, and windowed attention with sinks. Argument checks, the workspace plan, tensor
+// maps and launches; nothing here allocates device memory or synchronises.
+#include <string>
+
+#include <nvtx3/nvToolsExt.h>
+
+#include "internal.h"
+#include "norm_rope.cuh"
+#include "solb200.h"
+#include "window.cuh"
+
+using namespace solb200;
+
+namespace {
+
+struct NvtxRange {
+  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
+  ~NvtxRange() { nvtxRangePop(); }
+  NvtxRange(const NvtxRange&) = delete;
+  NvtxRange& operator=(const NvtxRange&) = delete;
+};
+
+int32_t invalid(const char* msg) { return set_last_error(SOLB200_ERR_INVALID, msg); }
+
+bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+constexpr int64_t kMost = (int64_t)1 << 30;
+
+// A [B, T, heads, D] tensor read with 16-byte accesses: base and the strides of dimensions
+// longer than one are multiples of 16 bytes (0 repeats the dimension).
+int32_t check_rows16(const char* name, const void* ptr, const int64_t* s, int64_t B, int64_t T, int64_t H, int esize,
+                     bool positive) {
+  if (!ptr || !s) return set_last_error(SOLB200_ERR_INVALID, std::string(name) + ": null pointer");
+  if (!aligned16(ptr))
+    return set_last_error(SOLB200_ERR_ALIGNMENT, std::string(name) + ": base not 16-byte aligned");
+  const int64_t n[3] = {B, T, H};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] < (positive ? 1 : 0) || s[i] > ((int64_t)1 << 40) || (s[i] * esize) % 16))
+      return set_last_error(SOLB200_ERR_ALIGNMENT,
+                            std::string(name) + ": batch/token/head strides must be multiples of 16 bytes" +
+                                (positive ? " above 0" : ", 0 or above"));
+  return SOLB200_OK;
+}
+
+// ------------------------------------------------------- head norms and rotation
+
+int32_t rope_params(RopeParams& p, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* wq,
+                    const void* wk, int32_t weight_dtype, const float* cos, const float* sin, const int64_t* ts,
+                    int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t R, int32_t dtype, float eps,
+                    int32_t interleaved) {
+  int32_t rc = check_sm100();
+  if (rc) return rc;
+  if (B < 1 || T < 1 || H < 1 || Hk < 1) return invalid("batch, tokens and heads must be >= 1");
+  if (B > kMost || T > kMost || H > 65536 || Hk > 65536) return invalid("batch, tokens or heads too large");
+  if (D < 8 || D > 256 || D % 8) return invalid("head_dim must be a multiple of 8 in [8, 256]");
+  if (dtype < 0 || dtype > 2) return invalid("dtype must be SOLB200_BF16, SOLB200_F16 or SOLB200_F32");
+  if (weight_dtype != dtype && weight_dtype != kDtypeF32)
+    return invalid("weights must have the tensors' dtype or be float32");
+  const int step = interleaved ? 8 : 16;
+  if (R < step || R > D || R % step)
+    return invalid("rotated elements must be a multiple of 8 (interleaved) or 16 (halves) in head_dim");
+  if (!(eps >= 0.f)) return invalid("eps must be >= 0");
+  const int es = dtype == kDtypeF32 ? 4 : 2;
+  if ((rc = check_rows16("q", q, qs, B, T, H, es, false))) return rc;
+  if ((rc = check_rows16("k", k, ks, B, T, Hk, es, false))) return rc;
+  if (!wq || !wk || !cos || !sin || !ts) return invalid("weights or tables: null pointer");
+  if (!aligned16(cos) || !aligned16(sin) || (B > 1 && (ts[0] % 4 || ts[0] < 0)) || (T > 1 && (ts[1] % 4 || ts[1] < 0)))
+    return set_last_error(SOLB200_ERR_ALIGNMENT, "cos / sin: base or row strides not multiples of 16 bytes");
+  p = RopeParams{};
+  p.t[0].x = q; p.t[0].weight = wq; p.t[0].heads = (int)H;
+  p.t[1].x = k; p.t[1].weight = wk; p.t[1].heads = (int)Hk;
+  for (int i = 0; i < 3; ++i) {
+    p.t[0].xs[i] = qs[i];
+    p.t[1].xs[i] = ks[i];
+  }
+  p.cos = cos; p.sin = sin; p.ts[0] = ts[0]; p.ts[1] = ts[1];
+  p.B = (int)B; p.T = (int)T; p.D = (int)D; p.R = (int)R; p.eps = eps;
+  return SOLB200_OK;
+}
+
+// ------------------------------------------------------------- windowed attention
+
+constexpr int kSlots = 148 * 2;   // forward CTAs resident on the GPU
+constexpr int kStepKeys = 64, kTileRows = 128;
+
+// Parts of the key axis. Alone, a tile's CTA takes one slot of the GPU for `steps` steps (the
+// most that the shapes and bounds allow; lengths live on the device) plus about kOpen steps'
+// time to open and close; parts make waves shorter where tiles are few, at the price of their
+// opening and of the joining kernel (kJoin steps' time). The cheapest count by that estimate.
+int window_splits(int64_t tiles, int64_t steps) {
+  constexpr int64_t kOpen = 3, kJoin = 6, kMostSplits = 64;
+  int best = 1;
+  int64_t best_cost = (tiles + kSlots - 1) / kSlots * (steps + kOpen);
+  for (int n = 2; n <= kMostSplits && n * 2 <= steps; ++n) {
+    const int64_t cost = (tiles * n + kSlots - 1) / kSlots * ((steps + n - 1) / n + kOpen) + kJoin;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
+struct WinPlan {
+  WinParams p;
+  int64_t off_ml, off_o, off_lse, off_delta, fwd_bytes, bwd_bytes;
+};
+
+int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, int64_t left,
+                    int64_t right, int64_t sinks) {
+  if (B < 1 || Tq < 1 || Tk < 1 || H < 1 || Hk < 1) return invalid("batch, tokens and heads must be >= 1");
+  if (D != 64 && D != 128) return invalid("head_dim must be 64 or 128");
+  if (B > 65536 || Tq > kMost || Tk > kMost || H > 65536) return invalid("batch, tokens or heads too large");
+  if (H % Hk || H / Hk > kTileRows) return invalid("heads must be a multiple of key heads, at most 128 times as many");
+  if (left < -1 || right < -1 || sinks < 0) return invalid("left and right must be >= -1 (-1: no bound), sinks >= 0");
+  WinParams& p = w.p;
+  p = WinParams{};
+  p.B = (int)B; p.Tq = (int)Tq; p.Tk = (int)Tk; p.H = (int)H; p.Hk = (int)Hk;
+  p.G = (int)(H / Hk);
+  p.TPT = kTileRows / p.G;
+  p.RT = p.TPT * p.G;
+  p.nqt = (int)((Tq + p.TPT - 1) / p.TPT);
+  p.nkt = (int)((Tk + kTileRows - 1) / kTileRows);
+  const int64_t far = (int64_t)1 << 40;   // past every position
+  p.left = left > far ? far : left;
+  p.right = right > far ? far : right;
+  p.sinks = (int)(sinks < Tk ? sinks : Tk);
+  const int64_t tiles = B * Hk * p.nqt;
+  if (tiles >= ((int64_t)1 << 24) || B * Hk * p.nkt >= ((int64_t)1 << 31)) return invalid("too many tiles");
+  int64_t keys = Tk;
+  if (left >= 0 && right >= 0 && left < Tk && right < Tk) {
+    const int64_t span = p.sinks + left + right + (Tq < p.TPT ? Tq : p.TPT);
+    if (span < keys) keys = span;
+  }
+  p.nsplit = window_splits(tiles, (keys + kStepKeys - 1) / kStepKeys + 1);
+  auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  int64_t cur = 256;   // the error word
+  w.off_ml = cur;
+  if (p.nsplit > 1) cur = up(cur + p.nsplit * B * Tq * H * (int64_t)sizeof(float2));
+  w.off_o = cur;
+  if (p.nsplit > 1) cur = up(cur + p.nsplit * B * Tq * H * D * (int64_t)sizeof(float));
+  w.fwd_bytes = cur;
+  const int64_t slots = tiles * kTileRows * (int64_t)sizeof(float);
+  w.off_lse = 256;
+  w.off_delta = w.off_lse + slots;
+  w.bwd_bytes = w.off_delta + slots;
+  return SOLB200_OK;
+}
+
+int32_t window_common(WinPlan& w, WinMaps& m, const void* q, const int64_t* qs, const void* k, const int64_t* ks,
+                      const void* v, const int64_t* vs, const int32_t* lengths, const int32_t* offsets, int64_t B,
+                      int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale, int key_box,
+                      void* workspace, int64_t workspace_bytes, int64_t need) {
+  int32_t rc;
+  if ((rc = check_rows16("q", q, qs, B, Tq, H, 2, true))) return rc;
+  if ((rc = check_rows16("k", k, ks, B, Tk, Hk, 2, true))) return rc;
+  if ((rc = check_rows16("v", v, vs, B, Tk, Hk, 2, true))) return rc;
+  if (!(scale > 0.f)) return invalid("scale must be > 0");
+  if (reinterpret_cast<uintptr_t>(lengths) % 4 || reinterpret_cast<uintptr_t>(offsets) % 4)
+    return set_last_error(SOLB200_ERR_ALIGNMENT, "lengths / offsets: not aligned to 4 bytes");
+  if (!workspace || workspace_bytes < need)
+    return set_last_error(SOLB200_ERR_WORKSPACE, "workspace missing or too small (" + std::to_string(workspace_bytes) +
+                                                     " of " + std::to_string(need) + " bytes)");
+  if (!aligned16(workspace)) return set_last_error(SOLB200_ERR_ALIGNMENT, "workspace not 16-byte aligned");
+  WinParams& p = w.p;
+  p.lengths = lengths;
+  p.offsets = offsets;
+  p.scale = scale;
+  p.s2 = scale * 1.4426950408889634f;
+  p.err = static_cast<int*>(workspace);
+  p.wait_ns = current_wait_ns();
+  if ((rc = bthd_map(&m.q, q, D, H, Tq, B, qs, p.G, p.TPT, "q"))) return rc;
+  if ((rc = bthd_map(&m.k, k, D, Hk, Tk, B, ks, 1, key_box, "k"))) return rc;
+  return bthd_map(&m.v, v, D, Hk, Tk, B, vs, 1, key_box, "v");
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t solb200_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             const void* q_weight, const void* k_weight, int32_t weight_dtype, const float* cos,
+                             const float* sin, const int64_t* table_strides, void* q_out, void* k_out, int64_t batch,
+                             int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotated,
+                             int32_t dtype, float eps, int32_t interleaved, void* stream) {
+  RopeParams p;
+  const int32_t rc = rope_params(p, q, q_strides, k, k_strides, q_weight, k_weight, weight_dtype, cos, sin,
+                                 table_strides, batch, tokens, heads, kv_heads, head_dim, rotated, dtype, eps,
+                                 interleaved);
+  if (rc) return rc;
+  if (!q_out || !k_out || !aligned16(q_out) || !aligned16(k_out))
+    return set_last_error(SOLB200_ERR_ALIGNMENT, "outputs: null or not 16-byte aligned");
+  p.t[0].out = q_out;
+  p.t[1].out = k_out;
+  NvtxRange r("solb200.qk_norm_rope");
+  const cudaError_t e = launch_norm_rope(p, dtype, weight_dtype, interleaved != 0, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "qk_norm_rope launch");
+}
+
+int32_t solb200_qk_norm_rope_backward_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t* bytes) {
+  if (!bytes) return invalid("null pointer");
+  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || batch > kMost || tokens > kMost || heads > 65536 ||
+      kv_heads > 65536)
+    return invalid("batch, tokens and heads must be >= 1");
+  if (head_dim < 8 || head_dim > 256 || head_dim % 8) return invalid("head_dim must be a multiple of 8 in [8, 256]");
+  *bytes = (int64_t)norm_rope_backward_ctas(batch, tokens, heads, kv_heads, (int)head_dim) * 2 * head_dim *
+           (int64_t)sizeof(float);
+  return SOLB200_OK;
+}
+
+int32_t solb200_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                                      const int64_t* dk_out_strides, const void* q, const int64_t* q_strides,
+                                      const void* k, const int64_t* k_strides, const void* q_weight,
+                                      const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                                      const int64_t* table_strides, void* dq, void* dk, void* dq_weight,
+                                      void* dk_weight, int64_t batch, int64_t tokens, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t rotated, int32_t dtype, float eps,
+                                      int32_t interleaved, void* workspace, int64_t workspace_bytes, void* stream) {
+  RopeParams p;
+  int32_t rc = rope_params(p, q, q_strides, k, k_strides, q_weight, k_weight, weight_dtype, cos, sin, table_strides,
+                           batch, tokens, heads, kv_heads, head_dim, rotated, dtype, eps, interleaved);
+  if (rc) return rc;
+  const int es = dtype == kDtypeF32 ? 4 : 2;
+  if ((rc = check_rows16("dq_out", dq_out, dq_out_strides, batch, tokens, heads, es, false))) return rc;
+  if ((rc = check_rows16("dk_out", dk_out, dk_out_strides, batch, tokens, kv_heads, es, false))) return rc;
+  if (!dq || !dk || !aligned16(dq) || !aligned16(dk) || !dq_weight || !dk_weight)
+    return set_last_error(SOLB200_ERR_ALIGNMENT, "gradients: null or not 16-byte aligned");
+  int64_t need = 0;
+  if ((rc = solb200_qk_norm_rope_backward_workspace(batch, tokens, heads, kv_heads, head_dim, &need))) return rc;
+  if (!workspace || workspace_bytes < need)
+    return set_last_error(SOLB200_ERR_WORKSPACE, "workspace missing or too small");
+  if (!aligned16(workspace)) return set_last_error(SOLB200_ERR_ALIGNMENT, "workspace not 16-byte aligned");
+  p.t[0].dy = dq_out; p.t[0].out = dq; p.t[0].dweight = dq_weight;
+  p.t[1].dy = dk_out; p.t[1].out = dk; p.t[1].dweight = dk_weight;
+  for (int i = 0; i < 3; ++i) {
+    p.t[0].dys[i] = dq_out_strides[i];
+    p.t[1].dys[i] = dk_out_strides[i];
+  }
+  p.partial = static_cast<float*>(workspace);
+  NvtxRange r("solb200.qk_norm_rope_backward");
+  const cudaError_t e =
+      launch_norm_rope_backward(p, dtype, weight_dtype, interleaved != 0, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "qk_norm_rope backward launch");
+}
+
+int32_t solb200_window_attn_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right, int64_t sinks,
+                                      int32_t backward, int64_t* bytes) {
+  if (!bytes) return invalid("null pointer");
+  WinPlan w;
+  const int32_t rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks);
+  if (rc) return rc;
+  *bytes = backward ? w.bwd_bytes : w.fwd_bytes;
+  return SOLB200_OK;
+}
+
+int32_t solb200_window_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                            const void* v, const int64_t* v_strides, void* out, float* lse, const int32_t* lengths,
+                            const int32_t* offsets, int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right, int64_t sinks,
+                            float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  int32_t rc = check_sm100();
+  if (rc) return rc;
+  WinPlan w;
+  WinMaps m;
+  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks))) return rc;
+  if (!out || !aligned16(out)) return set_last_error(SOLB200_ERR_ALIGNMENT, "out: null or not 16-byte aligned");
+  if ((rc = window_common(w, m, q, q_strides, k, k_strides, v, v_strides, lengths, offsets, batch, q_tokens,
+                          kv_tokens, heads, kv_heads, head_dim, scale, kStepKeys, workspace, workspace_bytes,
+                          w.fwd_bytes)))
+    return rc;
+  WinParams& p = w.p;
+  const int64_t os[3] = {q_tokens * heads * head_dim, heads * head_dim, head_dim};
+  if ((rc = bthd_map(&m.o, out, head_dim, heads, q_tokens, batch, os, p.G, p.TPT, "out"))) return rc;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + w.off_ml);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_o);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemsetAsync(p.err, 0, sizeof(int), st);
+  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemsetAsync(error word)");
+  NvtxRange r("solb200.window_attn");
+  e = launch_window_fwd((int)head_dim, m, p, st);
+  return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "window_attn launch");
+}
+
+int32_t solb200_window_attn_backward(const void* dout, const int64_t* dout_strides, const void* q,
+                                     const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                     const int64_t* v_strides, const void* out, const int64_t* out_strides,
+                                     const float* lse, void* dq, void* dk, void* dv, const int32_t* lengths,
+                                     const int32_t* offsets, int64_t batch, int64_t q_tokens, int64_t kv_tokens,
+                                     int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
+                                     int64_t sinks, float scale, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  int32_t rc = check_sm100();
+  if (rc) return rc;
+  WinPlan w;
+  WinMaps m;
+  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks))) return rc;
+  if ((rc = check_rows16("dout", dout, dout_strides, batch, q_tokens, heads, 2, true))) return rc;
+  if ((rc = check_rows16("out", out, out_strides, batch, q_tokens, heads, 2, true))) return rc;
+  if (!lse || !dq || !dk || !dv || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return set_last_error(SOLB200_ERR_ALIGNMENT, "lse or gradients: null or not 16-byte aligned");
+  if ((rc = window_common(w, m, q, q_strides, k, k_strides, v, v_strides, lengths, offsets, batch, q_tokens,
+                          kv_tokens, heads, kv_heads, head_dim, scale, kTileRows, workspace, workspace_bytes,
+                          w.bwd_bytes)))
+    return rc;
+  WinParams& p = w.p;
+  if ((rc = bthd_map(&m.dout, dout, head_dim, heads, q_tokens, batch, dout_strides, p.G, p.TPT, "dout"))) return rc;
+  p.out = static_cast<__nv_bfloat16*>(dq);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  p.lse_in = lse;
+  p.o_in = static_cast<const __nv_bfloat16*>(out);
+  p.do_in = static_cast<const __nv_bfloat16*>(dout);
+  for (int i = 0; i < 3; ++i) {
+    p.os[i] = out_strides[i];
+    p.dos[i] = dout_strides[i];
+  }
+  p.rows_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_lse);
+  p.rows_delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_delta);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemsetAsync(p.err, 0, sizeof(int), st);
+  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemsetAsync(error word)");
+  NvtxRange r("solb200.window_attn_backward");
+  e = launch_window_bwd((int)head_dim, m, p, st);
+  return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "window_attn backward launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,104 @@
+// Windowed attention with sinks (solb200_window_attn and its gradient): what query sees
+// which key, and the tiles that follow from it, shared by the kernels (window_fwd.cu,
+// window_bwd.cu) and the entry points (layer_api.cu).
+//
+// Query i of sequence b sits at position p = off_b + i. It sees key j when
+//   0 <= j < L_b,   j <= p + right,   and (j >= p - left or j < sinks).
+// The right bound holds for the sinks too, so a causal call (right = 0) stays causal.
+#pragma once
+
+#include "common.cuh"
+
+namespace solb200 {
+
+struct WinParams {
+  int B, Tq, Tk, H, Hk;
+  int G;                    // query heads per key head (H / Hk), 1..128
+  int TPT, RT, nqt;         // tokens and rows (TPT * G) of a query tile, tiles per (b, key head)
+  int nsplit;               // forward: parts of the key axis, joined by a second kernel
+  int64_t left, right;      // < 0: no bound
+  int sinks;
+  const int* lengths;       // [B] or null (Tk)
+  const int* offsets;       // [B] or null (L - Tq)
+  float scale, s2;          // softmax scale, and times log2(e)
+  int* err;
+  uint64_t wait_ns;
+  __nv_bfloat16* out;       // forward: dense [B, Tq, H, D]
+  float* lse;               // forward: [B, H, Tq] or null
+  float* part_o;            // split forward: [nsplit, B, Tq, H, D] unnormalised sums
+  float2* part_ml;          // split forward: [nsplit, B, Tq, H] (row maximum in log2 units, row sum)
+  // backward
+  const float* lse_in;      // [B, H, Tq]
+  const __nv_bfloat16 *o_in, *do_in;
+  int64_t os[3], dos[3];    // strides {batch, token, head}
+  float* rows_lse;          // [B, Hk, nqt, 128] lse * log2(e) by tile row (+inf: nothing seen, or no row)
+  float* rows_delta;        // [B, Hk, nqt, 128] sum(dO * O) by tile row
+  __nv_bfloat16 *dk, *dv;
+  int nkt;                  // key tiles of 128
+};
+
+// A sequence's place: valid keys and the position of query 0.
+struct WinSeq {
+  int L;
+  int64_t off;
+  __device__ WinSeq(const WinParams& p, int b) {
+    L = p.lengths ? min(max(__ldg(p.lengths + b), 0), p.Tk) : p.Tk;
+    off = p.offsets ? (int64_t)__ldg(p.offsets + b) : (int64_t)L - p.Tq;
+  }
+};
+
+__device__ __forceinline__ int clamp_to(int64_t x, int lo, int hi) {
+  return (int)(x < lo ? lo : (x > hi ? hi : x));
+}
+
+// First key past the right bound, and first key inside the left bound, of a query at `pos`.
+__device__ __forceinline__ int win_hi(const WinParams& p, int L, int64_t pos) {
+  return p.right < 0 ? L : clamp_to(pos + p.right + 1, 0, L);
+}
+__device__ __forceinline__ int win_lo(const WinParams& p, int64_t pos) {
+  return p.left < 0 ? 0 : clamp_to(pos - p.left, 0, p.Tk);
+}
+
+// The runs of STEP keys that the queries at positions [pa, pb] see any key of: steps
+// [0, n1) hold the sinks, steps [start, start + n - n1) the window.
+template <int STEP>
+struct WinSteps {
+  int n1, start, n;
+  __device__ WinSteps(const WinParams& p, int L, int64_t pa, int64_t pb) {
+    const int hi = win_hi(p, L, pb), lo = win_lo(p, pa);
+    const int end = (hi + STEP - 1) / STEP;
+    n1 = (min(p.sinks, hi) + STEP - 1) / STEP;
+    start = lo / STEP;
+    if (start <= n1) {
+      n1 = 0;
+      start = 0;
+      n = end;
+    } else {
+      n = n1 + max(0, end - start);
+    }
+  }
+  __device__ int key0(int s) const { return (s < n1 ? s : start + s - n1) * STEP; }
+};
+
+// Whether every query at positions [pa, pb] sees all of the keys [k0, k0 + n).
+__device__ __forceinline__ bool win_full(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
+  return k0 + n <= win_hi(p, L, pa) && (k0 >= win_lo(p, pb) || k0 + n <= p.sinks);
+}
+
+__device__ __forceinline__ uint32_t win_low_bits(int n) {
+  return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
+}
+
+// Bits of the 32 keys from k0 on that a query with bounds [lo, hi) sees.
+__device__ __forceinline__ uint32_t win_bits(int k0, int lo, int hi, int sinks) {
+  return win_low_bits(hi - k0) & (~win_low_bits(lo - k0) | win_low_bits(sinks - k0));
+}
+
+struct WinMaps {
+  CUtensorMap q, k, v, o, dout;
+};
+
+cudaError_t launch_window_fwd(int hd, const WinMaps& m, const WinParams& p, cudaStream_t st);
+cudaError_t launch_window_bwd(int hd, const WinMaps& m, const WinParams& p, cudaStream_t st);
+
+}  // namespace solb200

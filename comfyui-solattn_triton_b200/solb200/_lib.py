@@ -70,6 +70,20 @@ _SIGS = {
     "solb200_copy_heads": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                                      c_int32, c_void_p]),
     "solb200_selftest_quotient": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "solb200_qk_norm_rope": (c_int32, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p, c_void_p,
+                                       c_int32, c_void_p, c_void_p, POINTER(c_int64), c_void_p, c_void_p,
+                                       c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_float,
+                                       c_int32, c_void_p]),
+    "solb200_qk_norm_rope_backward_workspace": (c_int32, [c_int64] * 5 + [POINTER(c_int64)]),
+    "solb200_qk_norm_rope_backward": (c_int32, [c_void_p, POINTER(c_int64)] * 4
+                                      + [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, POINTER(c_int64)]
+                                      + [c_void_p] * 4 + [c_int64] * 6
+                                      + [c_int32, c_float, c_int32, c_void_p, c_int64, c_void_p]),
+    "solb200_window_attn_workspace": (c_int32, [c_int64] * 9 + [c_int32, POINTER(c_int64)]),
+    "solb200_window_attn": (c_int32, [c_void_p, POINTER(c_int64)] * 3 + [c_void_p] * 4 + [c_int64] * 9
+                            + [c_float, c_void_p, c_int64, c_void_p]),
+    "solb200_window_attn_backward": (c_int32, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p] * 6 + [c_int64] * 9
+                                     + [c_float, c_void_p, c_int64, c_void_p]),
     "solb200_gather_rows": (c_int32, [POINTER(c_void_p), POINTER(c_void_p), c_int32, c_void_p, c_int64,
                                       c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p]),
 }

@@ -265,6 +265,79 @@ SOLB200_API int32_t solb200_gather_rows(const void* const* src, void* const* dst
                             int64_t src_stride_b, int64_t src_stride_row, int64_t dst_stride_b,
                             int64_t dst_stride_row, void* stream);
 
+/* Element types of solb200_qk_norm_rope. */
+enum { SOLB200_BF16 = 0, SOLB200_F16 = 1, SOLB200_F32 = 2 };
+
+/* Root-mean-square norm of every head of q and k with the position rotation of the result,
+ * in one pass: n = x * w / sqrt(mean(x^2) + eps) over the head's head_dim elements, then the
+ * first `rotated` elements of the head are turned by the token's angles, (a, b) ->
+ * (a cos - b sin, a sin + b cos), on the pairs (2i, 2i + 1) if `interleaved`, else (i, i +
+ * rotated / 2). q: [batch, tokens, heads, head_dim], k: [.., kv_heads, ..], of `dtype`
+ * (SOLB200_BF16, _F16, _F32), strides {batch, token, head} in elements, multiples of 16 bytes
+ * (0 repeats a dimension). head_dim: a multiple of 8 up to 256; rotated: a multiple of 8
+ * (interleaved) or 16. q_weight / k_weight: head_dim contiguous elements of weight_dtype (that
+ * dtype or SOLB200_F32). cos / sin: fp32 rows of rotated / 2, strides table_strides {batch,
+ * token} (batch 0: one table for all). q_out / k_out: dense, of `dtype`; all arithmetic is in
+ * fp32. The reference receives q and k already normed and turned by the host's model. */
+SOLB200_API int32_t solb200_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k,
+                                         const int64_t* k_strides, const void* q_weight, const void* k_weight,
+                                         int32_t weight_dtype, const float* cos, const float* sin,
+                                         const int64_t* table_strides, void* q_out, void* k_out, int64_t batch,
+                                         int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t rotated, int32_t dtype, float eps, int32_t interleaved,
+                                         void* stream);
+
+/* Bytes of workspace for solb200_qk_norm_rope_backward with this geometry. */
+SOLB200_API int32_t solb200_qk_norm_rope_backward_workspace(int64_t batch, int64_t tokens, int64_t heads,
+                                                            int64_t kv_heads, int64_t head_dim, int64_t* bytes);
+
+/* Gradient of solb200_qk_norm_rope: from dq_out / dk_out (the gradients of its outputs,
+ * strided like q / k) and its inputs, dq / dk (dense, of `dtype`) and dq_weight / dk_weight (of
+ * weight_dtype; sums over all rows in fp32, in a fixed order: the same bits every time). */
+SOLB200_API int32_t solb200_qk_norm_rope_backward(
+    const void* dq_out, const int64_t* dq_out_strides, const void* dk_out, const int64_t* dk_out_strides,
+    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* q_weight,
+    const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin, const int64_t* table_strides,
+    void* dq, void* dk, void* dq_weight, void* dk_weight, int64_t batch, int64_t tokens, int64_t heads,
+    int64_t kv_heads, int64_t head_dim, int64_t rotated, int32_t dtype, float eps, int32_t interleaved,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace for solb200_window_attn (backward = 0) or its gradient (1). */
+SOLB200_API int32_t solb200_window_attn_workspace(int64_t batch, int64_t q_tokens, int64_t kv_tokens, int64_t heads,
+                                                  int64_t kv_heads, int64_t head_dim, int64_t left, int64_t right,
+                                                  int64_t sinks, int32_t backward, int64_t* bytes);
+
+/* Attention in a sliding window with a few first keys that stay visible (sinks). Query i of
+ * sequence b sits at position p = offsets[b] + i and sees key j when
+ *     0 <= j < lengths[b],  j <= p + right,  and  j >= p - left or j < sinks.
+ * left / right: -1 for no bound; right = 0 is causal, and holds for the sinks too. lengths
+ * (int32 [batch] on the device, nullable: kv_tokens) are clamped to [0, kv_tokens]; offsets
+ * (int32 [batch], nullable: lengths[b] - q_tokens, the last query at the last key). Keys past
+ * a length are not used and may hold anything, NaN included. A query that sees nothing gives
+ * zeros and lse = -inf.
+ * q: bf16 [batch, q_tokens, heads, head_dim], k / v: bf16 [batch, kv_tokens, kv_heads,
+ * head_dim], strides {batch, token, head} in elements, positive multiples of 8; head_dim 64 or
+ * 128; heads a multiple of kv_heads (query head h reads key head h / (heads / kv_heads)). out:
+ * dense bf16 like q. lse (nullable): fp32 [batch, heads, q_tokens], ln sum exp(scale q.k), for
+ * the gradient. One to a few query tokens against a long cache are split over the key axis.
+ * The workspace's first word is the device error word (solb200_read_device_error). */
+SOLB200_API int32_t solb200_window_attn(const void* q, const int64_t* q_strides, const void* k,
+                                        const int64_t* k_strides, const void* v, const int64_t* v_strides, void* out,
+                                        float* lse, const int32_t* lengths, const int32_t* offsets, int64_t batch,
+                                        int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads,
+                                        int64_t head_dim, int64_t left, int64_t right, int64_t sinks, float scale,
+                                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradient of solb200_window_attn: dq, dk, dv (dense bf16) from dout (strided like q) and the
+ * forward's inputs, out and lse, with its bounds. Keys that no query sees get zeros. Sums are
+ * in a fixed order: the same bits every time. q and dout have to be finite in every row. */
+SOLB200_API int32_t solb200_window_attn_backward(
+    const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides, const void* k,
+    const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides,
+    const float* lse, void* dq, void* dk, void* dv, const int32_t* lengths, const int32_t* offsets, int64_t batch,
+    int64_t q_tokens, int64_t kv_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t left,
+    int64_t right, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Self-test of the arithmetic of the int8 quantisers (no counterpart in the
  * reference): for n pairs (x[i], s[i]) of device float arrays (s > 0), adds to the
  * device counters bad[0] the pairs whose division-free quotient differs from the

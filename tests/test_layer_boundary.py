@@ -1,0 +1,67 @@
+"""The layer operators' refusals that need no GPU: status codes of the C ABI's planning calls,
+and the Python layer's refusal of host tensors."""
+
+import ctypes
+
+import pytest
+import torch
+
+import solb200
+from solb200 import _lib
+
+
+def _window_bytes(*args, backward=0):
+    n = ctypes.c_int64(-1)
+    return _lib.lib().solb200_window_attn_workspace(*args, backward, ctypes.byref(n)), n.value
+
+
+@pytest.mark.parametrize("args", [
+    (0, 4, 4, 2, 2, 64, -1, 0, 0),            # no sequence
+    (1, 0, 4, 2, 2, 64, -1, 0, 0),            # no query
+    (1, 4, 0, 2, 2, 64, -1, 0, 0),            # no key
+    (1, 4, 4, 2, 2, 96, -1, 0, 0),            # head_dim
+    (1, 4, 4, 3, 2, 64, -1, 0, 0),            # heads not a multiple
+    (1, 4, 4, 258, 2, 64, -1, 0, 0),          # more than 128 heads per key head
+    (1, 4, 4, 2, 2, 64, -2, 0, 0),            # bounds
+    (1, 4, 4, 2, 2, 64, -1, -2, 0),
+    (1, 4, 4, 2, 2, 64, -1, 0, -1),           # sinks
+    (1, 1 << 31, 4, 2, 2, 64, -1, 0, 0),      # lengths
+    (1, 4, 1 << 31, 2, 2, 64, -1, 0, 0),
+])
+def test_window_plan_refuses(args):
+    rc, n = _window_bytes(*args)
+    assert rc == 1 and n == -1 and _lib.last_error()
+
+
+def test_window_plan_splits_only_where_tiles_are_few():
+    rc, whole = _window_bytes(1, 32760, 32760, 40, 40, 128, 2340, 2340, 1560)
+    assert rc == 0 and whole == 256                      # fills the GPU: no parts
+    rc, token = _window_bytes(1, 1, 262144, 8, 8, 128, -1, 0, 0)
+    assert rc == 0 and token > 2 * 8 * (128 + 2) * 4     # several parts of one row per head
+    rc, short = _window_bytes(1, 1, 262144, 8, 8, 128, 30, 0, 0)
+    assert rc == 0 and short < token                     # a short window has few steps to divide
+    rc, huge = _window_bytes(1, 1, 262144, 8, 8, 128, (1 << 62), (1 << 62), 1 << 62)
+    assert rc == 0 and huge == token                     # bounds past every position
+    rc, grad = _window_bytes(2, 100, 100, 6, 2, 64, -1, 0, 0, backward=1)
+    assert rc == 0 and grad == 256 + 2 * 2 * 2 * 3 * 128 * 4   # two numbers per row of 3 tiles
+
+
+@pytest.mark.parametrize("args", [(0, 4, 2, 2, 64), (1, 0, 2, 2, 64), (1, 4, 0, 2, 64), (1, 4, 2, 0, 64),
+                                  (1, 4, 2, 2, 0), (1, 4, 2, 2, 60), (1, 4, 2, 2, 264)])
+def test_rope_plan_refuses(args):
+    n = ctypes.c_int64(-1)
+    assert _lib.lib().solb200_qk_norm_rope_backward_workspace(*args, ctypes.byref(n)) == 1
+    assert n.value == -1 and _lib.last_error()
+
+
+def test_host_tensors_are_refused():
+    q = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    w, t = torch.ones(64), torch.zeros(8, 32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        solb200.qk_norm_rope(q, q, w, w, t, t)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        solb200.qk_norm_rope_backward(q, q, q, q, w, w, t, t)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        solb200.window_attn(q, q, q)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        solb200.window_attn_backward(q, q, q, q, q, torch.zeros(1, 2, 8))
