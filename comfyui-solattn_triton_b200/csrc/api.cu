@@ -1,6 +1,7 @@
 // Host side of the C ABI (include/solb200.h): argument checks, the workspace plan,
 // TMA tensor maps and the launch sequence of each entry point. Nothing here
 // allocates device memory or synchronises, except solb200_read_device_error.
+#include <atomic>
 #include <mutex>
 #include <string>
 
@@ -675,7 +676,17 @@ int32_t set_last_error(int32_t code, const std::string& msg) { return fail(code,
 
 int32_t set_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 
-int32_t check_sm100() { return check_device(); }
+int32_t check_sm100() {
+  // devices that check_device() has accepted (their capability does not change)
+  static std::atomic<uint64_t> known{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 &&
+      (known.load(std::memory_order_relaxed) >> dev & 1))
+    return SOLB200_OK;
+  const int32_t rc = check_device();
+  if (rc == SOLB200_OK && dev >= 0 && dev < 64) known.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  return rc;
+}
 
 uint64_t current_wait_ns() { return g_debug_wait.wait_ns; }
 

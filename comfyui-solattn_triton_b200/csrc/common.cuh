@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #ifndef SOLB200_WAIT_NS
 #define SOLB200_WAIT_NS 2000000000ull   // 2 s: far above any legitimate wait
 #endif
@@ -66,6 +68,20 @@ inline cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, dim3 block, si
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
+}
+
+// Allow `smem` bytes of dynamic shared memory for a kernel on the current device, once per
+// device: `done` is the kernel's own bit mask of devices.
+template <typename Kern>
+inline cudaError_t allow_smem(Kern kern, size_t smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -254,6 +270,52 @@ __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// One lane of a converged warp (the same every time): 1 there, 0 in the others.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t mine;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(mine));
+  return mine;
+}
+
+// The products and the commit above for a whole converged warp, of which the lane with
+// `mine` issues. The operands stay warp-uniform, so they live in uniform registers: issued from
+// a single lane's branch, each product first moves its operands there (about 95 cycles
+// an instruction with four busy warps on the scheduler, against 64 of tensor-core time).
+__device__ __forceinline__ void mma_bf16_ss_warp(uint32_t mine, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(mine)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16_ts_warp(uint32_t mine, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(mine)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_warp(uint32_t mine, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(mine)
+      : "memory");
+}
+
 // Instruction descriptor (kind::f16 / kind::i8), dense, no negation.
 //   bits 4-5  D format (1 = f32, 2 = s32)   bits 7-9  A format   bits 10-12 B format
 //   bit 15    A major (0 = K-major)          bit 16    B major (1 = MN-major)
@@ -283,6 +345,9 @@ __device__ __forceinline__ uint64_t make_sw128_desc(uint32_t smem_addr, uint32_t
   d |= (uint64_t)2 << 61;
   return d;
 }
+
+// The same operand `bytes` further on (the address field cannot overflow inside shared memory).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 
 // TMEM loads / stores, 32 lanes x 32 bits shape: thread i of the warp reads/writes
 // lane (warp's lane quarter base + i), consecutive columns.
@@ -333,6 +398,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
       "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_ld() {

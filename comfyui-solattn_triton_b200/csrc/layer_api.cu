@@ -45,6 +45,11 @@ int32_t check_rows16(const char* name, const void* ptr, const int64_t* s, int64_
 
 // ------------------------------------------------------- head norms and rotation
 
+// batch x tokens x heads rows are numbered with 32-bit integers
+bool rope_rows_fit(int64_t B, int64_t T, int64_t H) {
+  return B <= kMost && T <= kMost && H <= 65536 && B * T <= kMost && B * T * H <= kMost;
+}
+
 int32_t rope_params(RopeParams& p, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* wq,
                     const void* wk, int32_t weight_dtype, const float* cos, const float* sin, const int64_t* ts,
                     int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t R, int32_t dtype, float eps,
@@ -52,7 +57,7 @@ int32_t rope_params(RopeParams& p, const void* q, const int64_t* qs, const void*
   int32_t rc = check_sm100();
   if (rc) return rc;
   if (B < 1 || T < 1 || H < 1 || Hk < 1) return invalid("batch, tokens and heads must be >= 1");
-  if (B > kMost || T > kMost || H > 65536 || Hk > 65536) return invalid("batch, tokens or heads too large");
+  if (!rope_rows_fit(B, T, H) || !rope_rows_fit(B, T, Hk)) return invalid("more than 2^30 rows in q or k");
   if (D < 8 || D > 256 || D % 8) return invalid("head_dim must be a multiple of 8 in [8, 256]");
   if (dtype < 0 || dtype > 2) return invalid("dtype must be SOLB200_BF16, SOLB200_F16 or SOLB200_F32");
   if (weight_dtype != dtype && weight_dtype != kDtypeF32)
@@ -201,11 +206,11 @@ int32_t solb200_qk_norm_rope(const void* q, const int64_t* q_strides, const void
 int32_t solb200_qk_norm_rope_backward_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                 int64_t head_dim, int64_t* bytes) {
   if (!bytes) return invalid("null pointer");
-  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1 || batch > kMost || tokens > kMost || heads > 65536 ||
-      kv_heads > 65536)
-    return invalid("batch, tokens and heads must be >= 1");
+  if (batch < 1 || tokens < 1 || heads < 1 || kv_heads < 1) return invalid("batch, tokens and heads must be >= 1");
+  if (!rope_rows_fit(batch, tokens, heads) || !rope_rows_fit(batch, tokens, kv_heads))
+    return invalid("more than 2^30 rows in q or k");
   if (head_dim < 8 || head_dim > 256 || head_dim % 8) return invalid("head_dim must be a multiple of 8 in [8, 256]");
-  *bytes = (int64_t)norm_rope_backward_ctas(batch, tokens, heads, kv_heads, (int)head_dim) * 2 * head_dim *
+  *bytes = (int64_t)norm_rope_backward_ctas(batch, tokens, heads, kv_heads, (int)head_dim) * head_dim *
            (int64_t)sizeof(float);
   return SOLB200_OK;
 }
@@ -278,11 +283,8 @@ int32_t solb200_window_attn(const void* q, const int64_t* q_strides, const void*
   p.lse = lse;
   p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + w.off_ml);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_o);
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemsetAsync(p.err, 0, sizeof(int), st);
-  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemsetAsync(error word)");
   NvtxRange r("solb200.window_attn");
-  e = launch_window_fwd((int)head_dim, m, p, st);
+  const cudaError_t e = launch_window_fwd((int)head_dim, m, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "window_attn launch");
 }
 
@@ -321,11 +323,8 @@ int32_t solb200_window_attn_backward(const void* dout, const int64_t* dout_strid
   }
   p.rows_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_lse);
   p.rows_delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_delta);
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemsetAsync(p.err, 0, sizeof(int), st);
-  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemsetAsync(error word)");
   NvtxRange r("solb200.window_attn_backward");
-  e = launch_window_bwd((int)head_dim, m, p, st);
+  const cudaError_t e = launch_window_bwd((int)head_dim, m, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SOLB200_OK : set_cuda_error(e, "window_attn backward launch");
 }
 

@@ -28,14 +28,14 @@ struct RopeParams {
   int64_t ts[2];        // table strides {batch, token}; a row holds R / 2 floats
   int B, T, D, R;
   float eps;
-  int chunks[2];        // items (runs of heads) per token of q and of k
-  int64_t items;        // B * T * (chunks[0] + chunks[1])
-  float* partial;       // backward: [CTAs, 2, D] sums of the weight gradients
+  int rows[2];          // B * T * heads
+  int ctas[2];          // CTAs that walk q's rows, then those that walk k's
+  float* partial;       // backward: [ctas[0] + ctas[1], D] sums of the weight gradients
 };
 
 cudaError_t launch_norm_rope(RopeParams p, int dtype, int wdtype, bool interleaved, cudaStream_t st);
 cudaError_t launch_norm_rope_backward(RopeParams p, int dtype, int wdtype, bool interleaved, cudaStream_t st);
-// CTAs of the backward pass for this geometry (the rows of RopeParams::partial)
+// CTAs of the backward pass for this geometry (the lines of RopeParams::partial)
 int norm_rope_backward_ctas(int64_t B, int64_t T, int64_t H, int64_t Hk, int D);
 
 }  // namespace solb200

@@ -94,6 +94,20 @@ __device__ __forceinline__ uint32_t win_bits(int k0, int lo, int hi, int sinks) 
   return win_low_bits(hi - k0) & (~win_low_bits(lo - k0) | win_low_bits(sinks - k0));
 }
 
+// Of the n keys from k0 on, those that no query at positions [pa, pb] sees: [a0, a1) between the
+// sinks and the window, [b0, n) past it. Their keys and values may hold anything, NaN included,
+// and 0 * NaN would reach the tile's sums: their rows are zeroed in shared memory.
+struct WinUnseen {
+  int a0, a1, b0;
+  __device__ WinUnseen(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
+    const int hi = win_hi(p, L, pb);
+    a0 = max(0, min(n, p.sinks - k0));
+    a1 = max(a0, min(n, win_lo(p, pa) - k0));
+    b0 = hi < p.Tk ? max(a1, min(n, hi - k0)) : n;   // (past Tk the loads fill in zeros)
+  }
+  __device__ bool any(int n) const { return a1 > a0 || b0 < n; }
+};
+
 struct WinMaps {
   CUtensorMap q, k, v, o, dout;
 };

@@ -11,11 +11,16 @@
 //   window_dq_kernel   a tile of 128 query rows; walks the 128-key steps of WinSteps: S and
 //                      dP, one query row per lane; dQ += dS K.
 // All products are M = 128, N = 128 (N = head_dim for the sums); sums stay in 32 bits in TMEM,
-// P and dS are rounded to bf16 for the tensor cores. 256 softmax threads (each 64 of a row's 128 columns),
-// one TMA warp, one MMA warp, one CTA per SM.
+// P and dS are rounded to bf16 for the tensor cores. 512 softmax threads (each 32 of a row's 128
+// columns: with 256 threads the chain of one thread's 64 columns, not a pipe, set the pace: 616 us
+// for window_dkv_kernel at 4 x 4096 tokens x 24 heads x 128, 1087 keys a row), one TMA warp, one MMA
+// warp, one CTA per SM.
 //
-// window_rows_kernel comes first: delta and -lse * log2(e) laid out by query tile, -inf for rows
-// that see nothing and for the tile's rows past the last token, which makes their P zero.
+// window_rows_kernel comes first: -delta and -lse * log2(e) laid out by query tile, -inf for rows
+// that see nothing and for the tile's rows past the last token, which makes their P zero. Its
+// delta carries the rounding of O to bf16, which counts where a row sees few keys (one key: dS
+// is exactly zero). For tiles of up to kFewSteps steps window_dq_kernel therefore forms delta =
+// sum(P dP) in 32 bits first, and leaves it for window_dkv_kernel.
 #include "fwd_common.cuh"
 #include "window.cuh"
 
@@ -25,28 +30,37 @@ namespace {
 
 constexpr int kTile = 128;
 constexpr uint32_t kBox = kTile * 128;   // a 128-row box of 64 bf16 columns
+constexpr int kSoftmax = 512;            // softmax threads: 4 per TMEM lane, 32 columns each
+constexpr int kThreads = kSoftmax + 64;
+constexpr int kFewSteps = 3;             // query tiles with up to this many key steps refine delta
 
 // D (128 x 128) = A B^T, both K-major in shared memory (HD columns).
 template <int HD>
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+__device__ __forceinline__ void mma_scores(uint32_t mine, uint32_t d, uint64_t a, uint64_t b) {
   constexpr uint32_t IDESC = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 0, 128, 128);
 #pragma unroll
   for (int k = 0; k < HD / 16; ++k) {
     const uint32_t o = (k >> 2) * kBox + (k & 3) * 32;
-    mma_bf16_ss(d, make_sw128_desc(a_smem + o, 16, 1024), make_sw128_desc(b_smem + o, 16, 1024), IDESC, k > 0);
+    mma_bf16_ss_warp(mine, d, desc_at(a, o), desc_at(b, o), IDESC, k > 0);
   }
 }
 
-// D (128 x HD) += A B, A bf16 in TMEM (rows 0-63 of the sum at a, rows 64-127 at a + 64), B
-// MN-major in shared memory (128 rows of HD columns).
+// D (128 x HD) += A B, A bf16 in TMEM (32 of the 128 summed rows at a, a + 32, a + 64, a + 96,
+// each in the columns that its softmax threads read the scores from), B MN-major in shared memory
+// (128 rows of HD columns).
 template <int HD>
-__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a, uint32_t b_smem, bool first) {
+__device__ __forceinline__ void mma_sum(uint32_t mine, uint32_t d, uint32_t a, uint64_t b, bool first) {
   constexpr uint32_t IDESC = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 1, 128, HD);
 #pragma unroll
   for (int k = 0; k < kTile / 16; ++k)
-    mma_bf16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, make_sw128_desc(b_smem + k * 2048, kBox, 1024), IDESC,
-                (first && k == 0) ? 0u : 1u);
+    mma_bf16_ts_warp(mine, d, a + (k >> 1) * 32 + (k & 1) * 8, desc_at(b, k * 2048), IDESC,
+                     (first && k == 0) ? 0u : 1u);
 }
+
+// Descriptors of a tile of 128 rows x HD columns: as a K-major operand (rows are M or N), and as
+// an MN-major one (rows are summed over).
+__device__ __forceinline__ uint64_t rows_desc(const uint8_t* tile) { return make_sw128_desc(smem_u32(tile), 16, 1024); }
+__device__ __forceinline__ uint64_t sum_desc(const uint8_t* tile) { return make_sw128_desc(smem_u32(tile), kBox, 1024); }
 
 // Zero rows [first, 128) of a tile of HD/64 boxes, by `n` threads.
 template <int HD>
@@ -84,6 +98,7 @@ __device__ __forceinline__ void store_row(uint32_t taddr, float scale, __nv_bflo
 template <int HD>
 __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WinParams p) {
   pdl_begin();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;   // the call's error word
   constexpr int GL = HD / 8;
   const int lg = threadIdx.x % GL;
   const int64_t slot = ((int64_t)blockIdx.x * 256 + threadIdx.x) / GL;   // [B, Hk, nqt, 128]
@@ -111,62 +126,51 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   for (int o = GL / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if (lg == 0 && b < p.B) {
     p.rows_lse[slot] = neg;
-    p.rows_delta[slot] = neg == -INFINITY ? 0.f : d;
+    p.rows_delta[slot] = neg == -INFINITY ? 0.f : -d;
   }
 }
 
-// 64 columns of P and dS for one TMEM lane. `nl(c)` and `dl(c)` give -lse * log2(e) and delta of
-// column c (0..63) - the same value for every column where a lane is a query row.
+// 32 columns of P for one TMEM lane: 2^(s * s2 - lse * log2(e)). `nl(i)` gives -lse * log2(e) of
+// columns i and i + 1 (where a lane is a query row, the same for all).
 template <bool MASKED, typename NL>
-__device__ __forceinline__ void probs(uint32_t t_s, float s2, uint32_t m0, uint32_t m1, float (&pr)[64], NL&& nl) {
-  uint32_t ra[32], rb[32];
-  tmem_ld32(t_s, ra);
-  tmem_ld32(t_s + 32, rb);
+__device__ __forceinline__ void probs(uint32_t t_s, float s2, uint32_t mask, float2 (&pr)[16], NL&& nl) {
+  uint32_t r[32];
+  tmem_ld32(t_s, r);
+  tmem_wait_ld();
+  const float2 s22 = make_float2(s2, s2);
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), s22, nl(i));
+    pr[i / 2] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+    if (MASKED) {
+      if (!((mask >> i) & 1u)) pr[i / 2].x = 0.f;
+      if (!((mask >> (i + 1)) & 1u)) pr[i / 2].y = 0.f;
+    }
+  }
+}
+
+__device__ __forceinline__ void store_cols(uint32_t t_out, const float2 (&x)[16]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(x[i].x, x[i].y);
+  tmem_st16(t_out, w);
+}
+
+// dP of the same columns. MASKED: a hidden key's dP may be anything, its P is 0.
+template <bool MASKED>
+__device__ __forceinline__ void load_dp(uint32_t t_dp, uint32_t mask, float2 (&dp)[16]) {
+  uint32_t r[32];
+  tmem_ld32(t_dp, r);
   tmem_wait_ld();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    pr[i] = fast_exp2(fmaf(__uint_as_float(ra[i]), s2, nl(i)));
-    pr[i + 32] = fast_exp2(fmaf(__uint_as_float(rb[i]), s2, nl(i + 32)));
-    if (MASKED) {
-      if (!((m0 >> i) & 1u)) pr[i] = 0.f;
-      if (!((m1 >> i) & 1u)) pr[i + 32] = 0.f;
-    }
-  }
-}
-
-template <bool MASKED, typename DL>
-__device__ __forceinline__ void score_grads(uint32_t t_dp, uint32_t t_out, uint32_t m0, uint32_t m1,
-                                            const float (&pr)[64], DL&& dl) {
+  for (int i = 0; i < 32; ++i)
+    if (MASKED && !((mask >> i) & 1u)) r[i] = 0u;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t r[32], w[16];
-    tmem_ld32(t_dp + c * 32, r);
-    tmem_wait_ld();
-    const uint32_t m = c ? m1 : m0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float g = pr[c * 32 + i] * (__uint_as_float(r[i]) - dl(c * 32 + i));
-      if (MASKED && !((m >> i) & 1u)) g = 0.f;   // a hidden key's dP may be anything
-      r[i] = __float_as_uint(g);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-    tmem_st16(t_out + c * 16, w);
-  }
-}
-
-__device__ __forceinline__ void store_probs(uint32_t t_out, const float (&pr)[64]) {
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(pr[c * 32 + 2 * i], pr[c * 32 + 2 * i + 1]);
-    tmem_st16(t_out + c * 16, w);
-  }
+  for (int i = 0; i < 16; ++i) dp[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 
 template <int HD>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                   const __grid_constant__ WinParams p) {
@@ -180,7 +184,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint8_t* sV = sK + TILE;
   uint8_t* sQ = sV + TILE;               // 2 stages
   uint8_t* sG = sQ + 2 * TILE;           // dO, 2 stages
-  float* sRow = reinterpret_cast<float*>(sG + 2 * TILE);   // 2 stages of [-lse2 128, delta 128]
+  float* sRow = reinterpret_cast<float*>(sG + 2 * TILE);   // 2 stages of [-lse2 128, -delta 128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 256);
   uint64_t* bar_kv = bars + 0;
   uint64_t* bar_q = bars + 1;            // [2] Q and its rows' numbers
@@ -194,7 +198,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* bar_drain = bars + 13;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
   // are seen by the most queries, and the longest CTAs start first
   int id = blockIdx.x;
@@ -207,7 +211,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
   const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
   const int q_begin = ta / p.TPT;
-  const int n = (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - q_begin : 0;
+  const int n = __shfl_sync(0xffffffffu, (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - q_begin : 0, 0);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_kv, 1);
@@ -218,20 +222,20 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(bar_dk + i, 1);
     }
     mbar_init(bar_s, 1);
-    mbar_init(bar_p, 256);
+    mbar_init(bar_p, kSoftmax);
     mbar_init(bar_dp, 1);
-    mbar_init(bar_ds, 256);
+    mbar_init(bar_ds, kSoftmax);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
   // rows that no box fills are summed over (with P = dS = 0): they have to be finite
   if (p.RT < kTile && n > 0)
     for (int i = 0; i < 2; ++i) {
-      zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, 320);
-      zero_rows<HD>(sG + i * TILE, p.RT, threadIdx.x, 320);
+      zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, kThreads);
+      zero_rows<HD>(sG + i * TILE, p.RT, threadIdx.x, kThreads);
     }
   fence_proxy_async_smem();
-  if (warp == 9) {
+  if (warp == kSoftmax / 32 + 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -241,7 +245,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t tmem = *tmem_slot;
   const uint32_t tS = tmem, tDP = tmem + 128, tDV = tmem + 256, tDK = tmem + 384;
 
-  if (warp == 8) {
+  if (warp == kSoftmax / 32) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
       mbar_arrive_expect_tx(bar_kv, 2 * TILE);
@@ -283,59 +287,57 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int i = max(0, last_g - 1); i <= last_g; ++i) mbar_wait(bar_g + (i & 1), (i >> 1) & 1, p.err, kErrWaitDrain);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
     //   S(0) dP(0) | dV(i) S(i+1) dK(i) dP(i+1) | ...  The softmax works on dS(i) while
     //   dV(i) and S(i+1) run, and on P(i+1) while dK(i) and dP(i+1) run.
-    if (lane == 0 && n > 0) {
-      const uint32_t k_s = smem_u32(sK), v_s = smem_u32(sV), q_s = smem_u32(sQ), g_s = smem_u32(sG);
-      bool ok = mbar_wait(bar_kv, 0, p.err, kErrWaitMma, p.wait_ns) &&
-                mbar_wait(bar_q, 0, p.err, kErrWaitMma, p.wait_ns);
-      if (ok) {
+    if (n > 0) {
+      const uint32_t mine = elect_one();
+      const uint64_t k_rows = rows_desc(sK), v_rows = rows_desc(sV), q_rows = rows_desc(sQ), g_rows = rows_desc(sG);
+      const uint64_t q_sum = sum_desc(sQ), g_sum = sum_desc(sG);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool done = mbar_wait_warp(bar, parity, p.err, kErrWaitMma, p.wait_ns);
         tc_fence_after();
-        mma_scores<HD>(tS, k_s, q_s);
-        tc_commit(bar_s);
-        ok = mbar_wait(bar_g, 0, p.err, kErrWaitMma, p.wait_ns);
+        return done;
+      };
+      bool ok = wait(bar_kv, 0) && wait(bar_q, 0);
+      if (ok) {
+        mma_scores<HD>(mine, tS, k_rows, q_rows);
+        tc_commit_warp(mine, bar_s);
+        ok = wait(bar_g, 0);
       }
       if (ok) {
-        tc_fence_after();
-        mma_scores<HD>(tDP, v_s, g_s);
-        tc_commit(bar_dp);
+        mma_scores<HD>(mine, tDP, v_rows, g_rows);
+        tc_commit_warp(mine, bar_dp);
       }
       for (int i = 0; ok && i < n; ++i) {
         const int st = i & 1, nx = st ^ 1;
         const uint32_t par = (i >> 1) & 1, npar = ((i + 1) >> 1) & 1;
-        if (!(ok = mbar_wait(bar_p, i & 1, p.err, kErrWaitMma, p.wait_ns))) break;
-        tc_fence_after();
-        mma_sum<HD>(tDV, tS, g_s + st * TILE, i == 0);
-        tc_commit(bar_dv + st);
+        if (!(ok = wait(bar_p, i & 1))) break;
+        mma_sum<HD>(mine, tDV, tS, desc_at(g_sum, st * TILE), i == 0);
+        tc_commit_warp(mine, bar_dv + st);
         if (i + 1 < n) {
           // S(i+1) overwrites P(i): dV(i) has to have read it
-          if (!(ok = mbar_wait(bar_q + nx, npar, p.err, kErrWaitMma, p.wait_ns))) break;
-          if (!(ok = mbar_wait(bar_dv + st, par, p.err, kErrWaitMma, p.wait_ns))) break;
-          tc_fence_after();
-          mma_scores<HD>(tS, k_s, q_s + nx * TILE);
-          tc_commit(bar_s);
+          if (!(ok = wait(bar_q + nx, npar) && wait(bar_dv + st, par))) break;
+          mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, nx * TILE));
+          tc_commit_warp(mine, bar_s);
         }
-        if (!(ok = mbar_wait(bar_ds, i & 1, p.err, kErrWaitMma, p.wait_ns))) break;
-        tc_fence_after();
-        mma_sum<HD>(tDK, tDP, q_s + st * TILE, i == 0);
-        tc_commit(bar_dk + st);
+        if (!(ok = wait(bar_ds, i & 1))) break;
+        mma_sum<HD>(mine, tDK, tDP, desc_at(q_sum, st * TILE), i == 0);
+        tc_commit_warp(mine, bar_dk + st);
         if (i + 1 < n) {
-          if (!(ok = mbar_wait(bar_g + nx, npar, p.err, kErrWaitMma, p.wait_ns))) break;
-          if (!(ok = mbar_wait(bar_dk + st, par, p.err, kErrWaitMma, p.wait_ns))) break;
-          tc_fence_after();
-          mma_scores<HD>(tDP, v_s, g_s + nx * TILE);
-          tc_commit(bar_dp);
+          if (!(ok = wait(bar_g + nx, npar) && wait(bar_dk + st, par))) break;
+          mma_scores<HD>(mine, tDP, v_rows, desc_at(g_rows, nx * TILE));
+          tc_commit_warp(mine, bar_dp);
         }
       }
-      // every MMA this thread issued has completed once bar_drain fires
-      tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, p.err, kErrWaitDrain);
+      // every product issued has completed once bar_drain fires
+      tc_commit_warp(mine, bar_drain);
+      mbar_wait_warp(bar_drain, 0, p.err, kErrWaitDrain);
     }
   } else {
     // -------------------------------------------- softmax + epilogue (one key per lane)
-    const int wg = warp >> 2, row = (warp & 3) * 32 + lane, c0 = wg * 64;
+    const int wg = warp >> 2, row = (warp & 3) * 32 + lane, c0 = wg * 32;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tS + lane_base + c0, tdp = tDP + lane_base + c0;
     const int j = j0 + row;
@@ -343,32 +345,34 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, t0 = (q_begin + i) * p.TPT;
       const int64_t pa = seq.off + t0, pb = pa + p.TPT - 1;
-      const float* neg = sRow + st * 256 + c0;
-      const float* delta = neg + 128;
+      const float2* neg = reinterpret_cast<const float2*>(sRow + st * 256 + c0);
+      const float2* ndelta = neg + 64;
       // every query of the tile sees every key of the tile?
       const bool full = j0 + kTile <= seq.L && (p.right < 0 || pa + p.right >= j0 + kTile - 1) &&
                         (p.left < 0 || pb - p.left <= j0 || j0 + kTile <= p.sinks);
-      uint32_t m0 = 0, m1 = 0;
+      uint32_t mask = 0;
       if (!full && j < seq.L) {
         const int lo = p.right < 0 ? 0 : clamp_to((int64_t)j - p.right - pa, 0, p.TPT) * p.G;
         const int hi = (p.left < 0 || j < p.sinks) ? kTile : clamp_to((int64_t)j + p.left - pa + 1, 0, p.TPT) * p.G;
-        m0 = win_low_bits(hi - c0) & ~win_low_bits(lo - c0);
-        m1 = win_low_bits(hi - c0 - 32) & ~win_low_bits(lo - c0 - 32);
+        mask = win_low_bits(hi - c0) & ~win_low_bits(lo - c0);
       }
       if (!(ok = mbar_wait_warp(bar_q + st, (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       if (!(ok = mbar_wait_warp(bar_s, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
-      float pr[64];
-      if (full) probs<false>(ts, p.s2, m0, m1, pr, [&](int c) { return neg[c]; });
-      else probs<true>(ts, p.s2, m0, m1, pr, [&](int c) { return neg[c]; });
-      store_probs(ts, pr);
+      float2 pr[16], dp[16];
+      if (full) probs<false>(ts, p.s2, mask, pr, [&](int c) { return neg[c / 2]; });
+      else probs<true>(ts, p.s2, mask, pr, [&](int c) { return neg[c / 2]; });
+      store_cols(ts, pr);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(bar_p);
       if (!(ok = mbar_wait_warp(bar_dp, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
-      if (full) score_grads<false>(tdp, tdp, m0, m1, pr, [&](int c) { return delta[c]; });
-      else score_grads<true>(tdp, tdp, m0, m1, pr, [&](int c) { return delta[c]; });
+      if (full) load_dp<false>(tdp, mask, dp);
+      else load_dp<true>(tdp, mask, dp);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) dp[c] = mul2(pr[c], add2(dp[c], ndelta[c]));
+      store_cols(tdp, dp);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(bar_ds);
@@ -376,20 +380,23 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok) {
-      __nv_bfloat16* dst = (wg ? p.dk : p.dv) + (((int64_t)b * p.Tk + j) * p.Hk + hk) * HD;
-      store_row<HD>((wg ? tDK : tDV) + lane_base, wg ? p.scale : 1.f, dst, j < p.Tk, n == 0);
+      // two of the four column groups store dV, two dK, half of the channels each
+      constexpr int NC = HD / 2;
+      const int half = (wg & 1) * NC;
+      __nv_bfloat16* dst = (wg < 2 ? p.dv : p.dk) + (((int64_t)b * p.Tk + j) * p.Hk + hk) * HD + half;
+      store_row<NC>((wg < 2 ? tDV : tDK) + lane_base + half, wg < 2 ? 1.f : p.scale, dst, j < p.Tk, n == 0);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kSoftmax / 32 + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
 template <int HD>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                  const __grid_constant__ WinParams p) {
@@ -414,7 +421,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* bar_drain = bars + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int id = blockIdx.x;
   const int qt = p.nqt - 1 - id % p.nqt;
   id /= p.nqt;
@@ -423,7 +430,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int t0 = qt * p.TPT, ntok = min(p.TPT, p.Tq - t0);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kTile> steps(p, seq.L, pa, pb);
-  const int n = steps.n, rows = ntok * p.G;
+  const int rows = ntok * p.G;
+  // passes over steps: with 2 .. kFewSteps steps, one pass for delta before the one for dS (a
+  // single step has all of a row's P and dP at hand)
+  const bool few = steps.n <= kFewSteps;
+  const int npre = __shfl_sync(0xffffffffu, few && steps.n > 1 ? steps.n : 0, 0);
+  const int n = __shfl_sync(0xffffffffu, npre + steps.n, 0);
+  auto key0 = [&](int i) { return steps.key0(i < npre ? i : i - npre); };
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
@@ -436,16 +449,16 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(bar_dp + i, 1);
       mbar_init(bar_s + i, 1);
     }
-    mbar_init(bar_ds, 256);
+    mbar_init(bar_ds, kSoftmax);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
   if (p.RT < kTile && n > 0) {
-    zero_rows<HD>(sQ, p.RT, threadIdx.x, 320);
-    zero_rows<HD>(sG, p.RT, threadIdx.x, 320);
+    zero_rows<HD>(sQ, p.RT, threadIdx.x, kThreads);
+    zero_rows<HD>(sG, p.RT, threadIdx.x, kThreads);
   }
   fence_proxy_async_smem();
-  if (warp == 9) {
+  if (warp == kSoftmax / 32 + 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -455,20 +468,20 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   const uint32_t tS = tmem, tDP = tmem + 256, tDQ = tmem + 384;   // two slots of S (dS written over them)
 
-  if (warp == 8) {
+  if (warp == kSoftmax / 32) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
       auto load_k = [&](int i) {
         uint64_t* bar = bar_k + i % 3;
         mbar_arrive_expect_tx(bar, TILE);
         for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sK + (i % 3) * TILE + x * kBox, &tm_k, bar, x * 64, hk, steps.key0(i), b);
+          tma_load_4d(sK + (i % 3) * TILE + x * kBox, &tm_k, bar, x * 64, hk, key0(i), b);
       };
       auto load_v = [&](int i) {
         uint64_t* bar = bar_v + (i & 1);
         mbar_arrive_expect_tx(bar, TILE);
         for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sV + (i & 1) * TILE + x * kBox, &tm_v, bar, x * 64, hk, steps.key0(i), b);
+          tma_load_4d(sV + (i & 1) * TILE + x * kBox, &tm_v, bar, x * 64, hk, key0(i), b);
       };
       mbar_arrive_expect_tx(bar_q, 2 * NBOX * p.RT * 128);
       for (int x = 0; x < NBOX; ++x) tma_load_4d(sQ + x * kBox, &tm_q, bar_q, x * 64, hk * p.G, t0, b);
@@ -496,96 +509,127 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         for (int i = max(0, last_v - 1); i <= last_v; ++i) mbar_wait(bar_v + (i & 1), (i >> 1) & 1, p.err, kErrWaitDrain);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
     //   S(0) dP(0) S(1) | dP(i+1) dQ(i) S(i+2) | ...
-    if (lane == 0 && n > 0) {
-      const uint32_t q_s = smem_u32(sQ), g_s = smem_u32(sG), k_s = smem_u32(sK), v_s = smem_u32(sV);
-      bool ok = mbar_wait(bar_q, 0, p.err, kErrWaitMma, p.wait_ns);
-      auto issue_s = [&](int i) {
-        ok = mbar_wait(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitMma, p.wait_ns);
-        if (!ok) return;
+    if (n > 0) {
+      const uint32_t mine = elect_one();
+      const uint64_t q_rows = rows_desc(sQ), g_rows = rows_desc(sG), k_rows = rows_desc(sK), v_rows = rows_desc(sV);
+      const uint64_t k_sum = sum_desc(sK);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool done = mbar_wait_warp(bar, parity, p.err, kErrWaitMma, p.wait_ns);
         tc_fence_after();
-        mma_scores<HD>(tS + (i & 1) * 128, q_s, k_s + (i % 3) * TILE);
-        tc_commit(bar_s + (i & 1));
+        return done;
+      };
+      auto issue_s = [&](int i) {
+        if (!wait(bar_k + i % 3, (i / 3) & 1)) return false;
+        mma_scores<HD>(mine, tS + (i & 1) * 128, q_rows, desc_at(k_rows, (i % 3) * TILE));
+        tc_commit_warp(mine, bar_s + (i & 1));
+        return true;
       };
       auto issue_dp = [&](int i) {
-        ok = mbar_wait(bar_v + (i & 1), (i >> 1) & 1, p.err, kErrWaitMma, p.wait_ns);
-        if (!ok) return;
-        tc_fence_after();
-        mma_scores<HD>(tDP, g_s, v_s + (i & 1) * TILE);
-        tc_commit(bar_dp + (i & 1));
+        if (!wait(bar_v + (i & 1), (i >> 1) & 1)) return false;
+        mma_scores<HD>(mine, tDP, g_rows, desc_at(v_rows, (i & 1) * TILE));
+        tc_commit_warp(mine, bar_dp + (i & 1));
+        return true;
       };
-      if (ok) issue_s(0);
-      if (ok) issue_dp(0);
-      if (ok && n > 1) issue_s(1);
+      bool ok = wait(bar_q, 0) && issue_s(0) && issue_dp(0) && (n == 1 || issue_s(1));
       for (int i = 0; ok && i < n; ++i) {
-        if (!(ok = mbar_wait(bar_ds, i & 1, p.err, kErrWaitMma, p.wait_ns))) break;
-        tc_fence_after();
-        if (i + 1 < n) issue_dp(i + 1);   // the softmax has taken dP(i) out
-        if (!ok) break;
-        mma_sum<HD>(tDQ, tS + (i & 1) * 128, k_s + (i % 3) * TILE, i == 0);
-        tc_commit(bar_dq + i % 3);
-        if (i + 2 < n) {
-          // S(i+2) overwrites dS(i): dQ(i) has to have read it
-          if (!(ok = mbar_wait(bar_dq + i % 3, (i / 3) & 1, p.err, kErrWaitMma, p.wait_ns))) break;
-          issue_s(i + 2);
-        }
+        // (the softmax has taken dP(i) out)
+        if (!(ok = wait(bar_ds, i & 1) && (i + 1 >= n || issue_dp(i + 1)))) break;
+        if (i >= npre) mma_sum<HD>(mine, tDQ, tS + (i & 1) * 128, desc_at(k_sum, (i % 3) * TILE), i == npre);
+        tc_commit_warp(mine, bar_dq + i % 3);
+        // S(i+2) overwrites dS(i): dQ(i) has to have read it
+        if (i + 2 < n) ok = wait(bar_dq + i % 3, (i / 3) & 1) && issue_s(i + 2);
       }
-      tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, p.err, kErrWaitDrain);
+      tc_commit_warp(mine, bar_drain);
+      mbar_wait_warp(bar_drain, 0, p.err, kErrWaitDrain);
     }
   } else {
     // ---------------------------------------- softmax + epilogue (one query row per lane)
-    const int wg = warp >> 2, row = (warp & 3) * 32 + lane, c0 = wg * 64;
+    const int wg = warp >> 2, row = (warp & 3) * 32 + lane, c0 = wg * 32;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int tok = row / p.G, head = row - tok * p.G;
     const bool live = row < rows;
     const int64_t pos = pa + tok;
     const int hi = live ? win_hi(p, seq.L, pos) : 0, lo = live ? win_lo(p, pos) : 0;
     const int64_t slot = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile + row;
-    const float neg = p.rows_lse[slot], delta = p.rows_delta[slot];
+    const float neg = p.rows_lse[slot];
+    float ndelta = p.rows_delta[slot];
+    float sum = 0.f;   // of P dP over this thread's columns, for delta
+    // delta of the row from its four threads' parts, for this kernel and for window_dkv_kernel; the
+    // parts meet in dQ's columns, which the first dQ product overwrites later
+    auto refine = [&]() {
+      tmem_st1(tDQ + lane_base + wg, __float_as_uint(sum));
+      tmem_wait_st();
+      tc_fence_before();
+      named_bar_sync(1, kSoftmax);
+      tc_fence_after();
+      uint32_t r[4];
+      tmem_ld4(tDQ + lane_base, r);
+      tmem_wait_ld();
+      ndelta = -((__uint_as_float(r[0]) + __uint_as_float(r[1])) + (__uint_as_float(r[2]) + __uint_as_float(r[3])));
+      if (wg == 0) p.rows_delta[slot] = ndelta;
+    };
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const int k0 = steps.key0(i);
+      const int k0 = key0(i);
       const uint32_t ts = tS + (i & 1) * 128 + lane_base + c0, tdp = tDP + lane_base + c0;
       const bool full = win_full(p, seq.L, pa, pb, k0, kTile);
-      uint32_t m0 = 0, m1 = 0;
-      if (!full && live) {
-        m0 = win_bits(k0 + c0, lo, hi, p.sinks);
-        m1 = win_bits(k0 + c0 + 32, lo, hi, p.sinks);
-      }
-      if (!(ok = mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+      const uint32_t mask = !full && live ? win_bits(k0 + c0, lo, hi, p.sinks) : 0u;
+      ok = mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
       tc_fence_after();
-      float pr[64];
-      if (full) probs<false>(ts, p.s2, m0, m1, pr, [&](int) { return neg; });
-      else probs<true>(ts, p.s2, m0, m1, pr, [&](int) { return neg; });
-      if (!(ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
-      tc_fence_after();
-      if (full) score_grads<false>(tdp, ts, m0, m1, pr, [&](int) { return delta; });
-      else score_grads<true>(tdp, ts, m0, m1, pr, [&](int) { return delta; });
-      if (k0 + kTile > seq.L && seq.L < p.Tk) {
-        // keys past the sequence's length may hold anything: zero their rows for dS K
-        // (S(i) is complete, and bar_k was waited for before it was issued)
-        if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
-        zero_rows<HD>(sK + (i % 3) * TILE, seq.L - k0, threadIdx.x, 256);
-        fence_proxy_async_smem();
+      float2 pr[16], dp[16];
+      if (ok) {
+        if (full) probs<false>(ts, p.s2, mask, pr, [&](int) { return make_float2(neg, neg); });
+        else probs<true>(ts, p.s2, mask, pr, [&](int) { return make_float2(neg, neg); });
+        ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
+        tc_fence_after();
       }
-      tmem_wait_st();
+      if (ok) {
+        if (full) load_dp<false>(tdp, mask, dp);
+        else load_dp<true>(tdp, mask, dp);
+      }
+      if (few) {
+        if (ok && (i < npre || n == 1))
+#pragma unroll
+          for (int c = 0; c < 16; ++c) sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
+        // (every softmax thread comes here at these steps: a failed wait leaves the loop only below)
+        if (n == 1 || i + 1 == npre) refine();
+      }
+      if (!ok) break;
+      if (i >= npre) {
+        const float2 nd = make_float2(ndelta, ndelta);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) dp[c] = mul2(pr[c], add2(dp[c], nd));
+        store_cols(ts, dp);
+        const WinUnseen unseen(p, seq.L, pa, pb, k0, kTile);
+        if (!full && unseen.any(kTile)) {
+          // (S(i) is complete, and bar_k was waited for before it was issued)
+          if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+          uint8_t* tile = sK + (i % 3) * TILE;
+          for (int c = threadIdx.x; c < kTile * NBOX * 8; c += kSoftmax) {
+            const int r = c / (NBOX * 8), x = c % (NBOX * 8);
+            if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
+              *reinterpret_cast<uint4*>(tile + (x >> 3) * kBox + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+      }
       tc_fence_before();
       mbar_arrive(bar_ds);
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
-    if (ok) {
-      constexpr int NC = HD / 2;
+    if (ok && wg < HD / 32) {
       const int64_t orow = ((int64_t)b * p.Tq + t0 + tok) * p.H + hk * p.G + head;
-      store_row<NC>(tDQ + lane_base + wg * NC, p.scale, p.out + orow * HD + wg * NC, live, n == 0);
+      store_row<32>(tDQ + lane_base + wg * 32, p.scale, p.out + orow * HD + wg * 32, live, n == 0);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kSoftmax / 32 + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -595,18 +639,19 @@ template <int HD>
 cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   constexpr size_t TILE = (HD / 64) * kBox;
   constexpr size_t smem_kv = 6 * TILE + 2048 + 128 + 1024, smem_q = 7 * TILE + 128 + 1024;
-  cudaError_t e = cudaFuncSetAttribute(window_dkv_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_kv);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(window_dq_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_q);
+  static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
+  cudaError_t e = allow_smem(window_dkv_kernel<HD>, smem_kv, allowed_kv);
+  if (e == cudaSuccess) e = allow_smem(window_dq_kernel<HD>, smem_q, allowed_q);
   if (e != cudaSuccess) return e;
   const int64_t slots = (int64_t)p.B * p.Hk * p.nqt * kTile;
   e = launch_pdl(window_rows_kernel<HD>, dim3((unsigned)(slots * (HD / 8) / 256)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(window_dkv_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nkt)), dim3(320), smem_kv, st, m.q, m.k,
-                 m.v, m.dout, p);
+  // window_dq_kernel leaves refined deltas for window_dkv_kernel
+  e = launch_pdl(window_dq_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nqt)), dim3(kThreads), smem_q, st, m.q,
+                 m.k, m.v, m.dout, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(window_dq_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nqt)), dim3(320), smem_q, st, m.q, m.k,
-                    m.v, m.dout, p);
+  return launch_pdl(window_dkv_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nkt)), dim3(kThreads), smem_kv, st,
+                    m.q, m.k, m.v, m.dout, p);
 }
 
 }  // namespace

@@ -17,8 +17,7 @@
 // cache), the steps are divided over nsplit CTAs, which write their unnormalised sums, maxima
 // and row sums; join_kernel joins them in order.
 //
-// Keys past a sequence's length may hold anything: their scores are replaced, and their
-// rows of V are zeroed in shared memory, so that 0 * NaN cannot reach the sums.
+// Keys that no row of the tile sees may hold anything (WinUnseen).
 #include "fwd_common.cuh"
 #include "window.cuh"
 
@@ -75,6 +74,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int active = (rows + 31) / 32;             // softmax warps that hold any
 
   if (threadIdx.x == 0) {
+    // the call's error word: nothing else writes it until a wait of some CTA runs out
+    if (blockIdx.x == 0) *p.err = 0;
     mbar_init(bar_q, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_kfull + i, 1);
@@ -208,13 +209,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           bits[0] = live ? win_bits(k0, lo, hi, p.sinks) : 0u;
           bits[1] = live ? win_bits(k0 + 32, lo, hi, p.sinks) : 0u;
           softmax_half<true, false, HD>(ts, tO + lane_base, bits, p.s2, m_ref, l_sum, s > 0, -1, 0.f, 1.f, drain);
-          if (ok && k0 + kStep > seq.L && seq.L < p.Tk) {
-            // keys past the sequence's length: zero their rows of V
+          const WinUnseen unseen(p, seq.L, pa, pb, k0, kStep);
+          if (ok && unseen.any(kStep)) {
             if ((ok = mbar_wait_warp(bar_vfull + slot, (s >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) {
-              const int first = max(0, seq.L - k0), n = (kStep - first) * 8;
-              for (int i = row; i < NBOX * n; i += 32 * active)
-                *reinterpret_cast<uint4*>(sV + slot * SLOT + (i / n) * HBOX + first * 128 + (i % n) * 16) =
-                    make_uint4(0, 0, 0, 0);
+              for (int i = row; i < kStep * NBOX * 8; i += 32 * active) {
+                const int r = i / (NBOX * 8), x = i % (NBOX * 8);
+                if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
+                  *reinterpret_cast<uint4*>(sV + slot * SLOT + (x >> 3) * HBOX + r * 128 + (x & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+              }
               fence_proxy_async_smem();
             }
           }
@@ -345,7 +348,8 @@ cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   // at least ~100 KB, so that at most two CTAs (512 TMEM columns) share an SM
   constexpr size_t need = (HD / 64) * (128 * 128 + 4 * kStep * 128) + 256 + 1024;
   const size_t smem = need < 100 * 1024 ? 100 * 1024 : need;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   const int64_t grid = (int64_t)p.B * p.Hk * p.nqt * p.nsplit;
   e = launch_pdl(kern, dim3((unsigned)grid), dim3(192), smem, st, m.q, m.k, m.v, m.o, p);

@@ -17,12 +17,12 @@ from __future__ import annotations
 import ctypes
 from contextlib import nullcontext
 from ctypes import c_int32, c_int64
-from functools import lru_cache
+from types import SimpleNamespace
 
 import torch
 
 from ._lib import I64x2, I64x3, check, lib
-from .ops import _SYNC_CHECK, _stream_ptr
+from .ops import _SYNC_CHECK
 
 # element types as the C ABI numbers them (SOLB200_BF16, _F16, _F32)
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -32,9 +32,29 @@ def _refuse(what):
     raise RuntimeError(f"solb200: {what}")
 
 
-def _on(device):
-    """A context in which `device` is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_HERE = nullcontext()
+_device_now = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream's handle, by device index
+
+
+def _on(index):
+    """A context in which device `index` is current."""
+    return _HERE if index == _device_now() else torch.cuda.device(index)
+
+
+# What a call's shapes, strides, types and options determine (the checks passed, output shapes,
+# stride arrays, workspace sizes), by those alone: a repeated geometry skips the checks.
+_PLANS = {}
+
+
+def _plan(key, make, *args):
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = make(*args)
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
 
 
 def _rows16(t, broadcast):
@@ -69,18 +89,27 @@ def _strides(t):
     return I64x3(s[0], s[1], s[2])
 
 
+def _in_place(t, broadcast):
+    """Whether `t`'s rows can be read with 16-byte accesses where they lie, its base aside."""
+    step = 16 // t.element_size()
+    return t.stride(-1) == 1 and not any(n > 1 and (s % step or (s == 0 and not broadcast))
+                                         for n, s in zip(t.shape[:-1], t.stride()))
+
+
 # ------------------------------------------------------- head norms and rotation
 
 
-def _rope_check(q, k, q_weight, k_weight, cos, sin, interleaved):
-    """Checked and packed arguments: (q, k, weights, tables, table strides)."""
+def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
     if q.dtype not in DTYPES:
         _refuse(f"q must be bfloat16, float16 or float32 (got {q.dtype})")
     _bthd(q, "q", q.dtype, q.device)
     _bthd(k, "k", q.dtype, q.device)
     B, T, H, D = q.shape
+    Hk = k.shape[2]
     if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
         _refuse(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head_dim")
+    if (H == 0) != (Hk == 0):
+        _refuse("q and k must both have heads")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w.shape != (D,) or w.device != q.device:
             _refuse(f"{name} must be one element per channel of a head, [{D}] on {q.device}")
@@ -96,61 +125,74 @@ def _rope_check(q, k, q_weight, k_weight, cos, sin, interleaved):
     step = 8 if interleaved else 16
     if D % 8 or not 8 <= D <= 256 or R % step or not step <= R <= D:
         _refuse(f"head_dim {D} must be a multiple of 8 up to 256, and {R} rotated elements a multiple of {step} in it")
+    if not eps >= 0:
+        _refuse(f"eps must be >= 0, got {eps}")
+    n = c_int64(0)
+    if B and T and H:
+        check(lib().solb200_qk_norm_rope_backward_workspace(B, T, H, Hk, D, ctypes.byref(n)), "workspace")
+    return SimpleNamespace(
+        place=(B, T, H, Hk, D, R, DTYPES[q.dtype], float(eps), int(bool(interleaved))), empty=not (B and T and H),
+        wtype=DTYPES[q_weight.dtype], qs=_strides(q), ks=_strides(k), backward_bytes=n.value,
+        ts=I64x2(0, cos.stride(0)) if cos.dim() == 2 else I64x2(cos.stride(0), cos.stride(1)),
+        in_place=(_in_place(q, True) and _in_place(k, True) and _in_place(cos, True) and cos.stride() == sin.stride()
+                  and q_weight.is_contiguous() and k_weight.is_contiguous()))
+
+
+def _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
+    """(plan, tensors): the tensors as the kernels can read them, packed where they have to be."""
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
+           q_weight.shape, q_weight.stride(), q_weight.dtype, q_weight.get_device(), k_weight.shape,
+           k_weight.stride(), k_weight.dtype, k_weight.get_device(), cos.shape, cos.stride(), cos.dtype,
+           cos.get_device(), sin.shape, sin.stride(), sin.dtype, sin.get_device(), eps, interleaved)
+    plan = _PLANS.get(key) or _plan(key, _rope_plan, q, k, q_weight, k_weight, cos, sin, eps, interleaved)
+    if plan.in_place and not (q.data_ptr() | k.data_ptr() | cos.data_ptr() | sin.data_ptr()) & 15:
+        return plan, q, k, q_weight, k_weight, cos, sin
+    q, k, q_weight, k_weight = _rows16(q, True), _rows16(k, True), q_weight.contiguous(), k_weight.contiguous()
     cos, sin = _rows16(cos, True), _rows16(sin, True)
     if cos.stride() != sin.stride():
-        cos, sin = cos.contiguous(), sin.contiguous()
-    ts = I64x2(0, cos.stride(0)) if cos.dim() == 2 else I64x2(cos.stride(0), cos.stride(1))
-    return (_rows16(q, True), _rows16(k, True), q_weight.contiguous(), k_weight.contiguous(), cos, sin, ts, R)
+        cos, sin = _rows16(cos.contiguous(), True), _rows16(sin.contiguous(), True)
+    return _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved), q, k, q_weight, k_weight, cos, sin
 
 
 def _rope_forward(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
-    q, k, wq, wk, cos, sin, ts, R = _rope_check(q, k, q_weight, k_weight, cos, sin, interleaved)
-    B, T, H, D = q.shape
-    q_out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-    k_out = torch.empty((B, T, k.shape[2], D), dtype=q.dtype, device=q.device)
-    if q.numel() and k.numel():
-        with _on(q.device):
-            check(lib().solb200_qk_norm_rope(
-                q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), DTYPES[wq.dtype],
-                cos.data_ptr(), sin.data_ptr(), ts, q_out.data_ptr(), k_out.data_ptr(), B, T, H, k.shape[2], D, R,
-                DTYPES[q.dtype], eps, int(interleaved), _stream_ptr(q.device)), "qk_norm_rope")
-    elif q.numel() or k.numel():
-        _refuse("q and k must both have heads")
+    plan, q, k, wq, wk, cos, sin = _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
+    B, T, H, Hk, D = plan.place[:5]
+    q_out, k_out = q.new_empty((B, T, H, D)), q.new_empty((B, T, Hk, D))
+    if not plan.empty:
+        index = q.get_device()
+        with _on(index):
+            rc = lib().solb200_qk_norm_rope(
+                q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, wq.data_ptr(), wk.data_ptr(), plan.wtype, cos.data_ptr(),
+                sin.data_ptr(), plan.ts, q_out.data_ptr(), k_out.data_ptr(), *plan.place, _raw_stream(index))
+        if rc:
+            check(rc, "qk_norm_rope")
     return q_out, k_out
-
-
-@lru_cache(maxsize=256)
-def _rope_workspace(B, T, H, Hk, D):
-    n = c_int64(0)
-    check(lib().solb200_qk_norm_rope_backward_workspace(B, T, H, Hk, D, ctypes.byref(n)), "workspace")
-    return n.value
 
 
 def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, eps=1e-6, interleaved=True):
     """(dq, dk, dq_weight, dk_weight) from the gradients of ``qk_norm_rope``'s outputs and its
     inputs. The weights' gradients are summed in fp32 in a fixed order."""
-    q, k, wq, wk, cos, sin, ts, R = _rope_check(q, k, q_weight, k_weight, cos, sin, interleaved)
-    _bthd(dq_out, "dq_out", q.dtype, q.device, q.shape)
-    _bthd(dk_out, "dk_out", q.dtype, q.device, k.shape)
+    plan, q, k, wq, wk, cos, sin = _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
+    for g, x, name in ((dq_out, q, "dq_out"), (dk_out, k, "dk_out")):
+        if g.shape != x.shape or g.dtype != x.dtype or g.get_device() != x.get_device():
+            _bthd(g, name, x.dtype, x.device, x.shape)
     dq_out, dk_out = _rows16(dq_out, True), _rows16(dk_out, True)
-    B, T, H, D = q.shape
-    Hk = k.shape[2]
-    dq = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-    if not (q.numel() and k.numel()):
-        if q.numel() or k.numel():
-            _refuse("q and k must both have heads")
+    B, T, H, Hk, D = plan.place[:5]
+    dq, dk = q.new_empty((B, T, H, D)), q.new_empty((B, T, Hk, D))
+    if plan.empty:
         return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk)
-    dw = torch.empty((2, D), dtype=wq.dtype, device=q.device)
-    with _on(q.device):
-        n = _rope_workspace(B, T, H, Hk, D)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        check(lib().solb200_qk_norm_rope_backward(
-            dq_out.data_ptr(), _strides(dq_out), dk_out.data_ptr(), _strides(dk_out), q.data_ptr(), _strides(q),
-            k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), DTYPES[wq.dtype], cos.data_ptr(), sin.data_ptr(),
-            ts, dq.data_ptr(), dk.data_ptr(), dw.data_ptr(), dw.data_ptr() + D * dw.element_size(), B, T, H, Hk, D, R,
-            DTYPES[q.dtype], eps, int(interleaved), ws.data_ptr(), n, _stream_ptr(q.device)), "qk_norm_rope_backward")
-    return dq, dk, dw[0], dw[1]
+    dwq, dwk = wq.new_empty(D), wq.new_empty(D)
+    index = q.get_device()
+    with _on(index):
+        ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=q.device)
+        rc = lib().solb200_qk_norm_rope_backward(
+            dq_out.data_ptr(), _strides(dq_out), dk_out.data_ptr(), _strides(dk_out), q.data_ptr(), plan.qs,
+            k.data_ptr(), plan.ks, wq.data_ptr(), wk.data_ptr(), plan.wtype, cos.data_ptr(), sin.data_ptr(), plan.ts,
+            dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), *plan.place, ws.data_ptr(),
+            plan.backward_bytes, _raw_stream(index))
+    if rc:
+        check(rc, "qk_norm_rope_backward")
+    return dq, dk, dwq, dwk
 
 
 class _NormRope(torch.autograd.Function):
@@ -177,19 +219,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, eps=1e-6, interleaved=Tr
                                     or k_weight.requires_grad or cos.requires_grad or sin.requires_grad):
         if cos.requires_grad or sin.requires_grad:
             _refuse("cos and sin take no gradient")
-        return _NormRope.apply(q, k, q_weight, k_weight, cos, sin, float(eps), bool(interleaved))
-    return _rope_forward(q, k, q_weight, k_weight, cos, sin, float(eps), bool(interleaved))
+        return _NormRope.apply(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
+    return _rope_forward(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
 
 
 # ------------------------------------------------------------- windowed attention
-
-
-@lru_cache(maxsize=1024)
-def _window_workspace(B, Tq, Tk, H, Hk, D, left, right, sinks, backward):
-    n = c_int64(0)
-    check(lib().solb200_window_attn_workspace(B, Tq, Tk, H, Hk, D, left, right, sinks, backward, ctypes.byref(n)),
-          "window_attn workspace")
-    return n.value
 
 
 def _bound(x, name):
@@ -197,18 +231,10 @@ def _bound(x, name):
         return -1
     if x < 0:
         _refuse(f"{name} must be None (no bound) or >= 0, got {x}")
-    return int(x)
+    return min(int(x), 1 << 40)                # past every position
 
 
-def _per_sequence(t, name, B, device):
-    if t is None:
-        return None
-    if not torch.is_tensor(t) or t.dtype != torch.int32 or t.shape != (B,) or t.device != device:
-        _refuse(f"{name} must be an int32 tensor of one number per sequence, [{B}] on {device}")
-    return t.contiguous()
-
-
-def _window_check(q, k, v, left, right, sinks, scale, lengths, offsets):
+def _window_plan(q, k, v, left, right, sinks, scale):
     _bthd(q, "q", torch.bfloat16, q.device)
     _bthd(k, "k", torch.bfloat16, q.device)
     _bthd(v, "v", torch.bfloat16, q.device, k.shape)
@@ -225,38 +251,65 @@ def _window_check(q, k, v, left, right, sinks, scale, lengths, offsets):
     scale = D ** -0.5 if scale is None else float(scale)
     if not scale > 0:
         _refuse(f"scale must be > 0, got {scale}")
-    bounds = (_bound(left, "left"), _bound(right, "right"), int(sinks))
-    return bounds, scale, _per_sequence(lengths, "lengths", B, q.device), _per_sequence(offsets, "offsets", B, q.device)
+    bounds = (_bound(left, "left"), _bound(right, "right"), min(int(sinks), 1 << 40))
+    empty = not (B and Tq and Tk and H)
+    n = [c_int64(0), c_int64(0)]
+    if not empty:
+        for backward in (0, 1):
+            check(lib().solb200_window_attn_workspace(B, Tq, Tk, H, Hk, D, *bounds, backward,
+                                                      ctypes.byref(n[backward])), "window_attn workspace")
+    return SimpleNamespace(place=(B, Tq, Tk, H, Hk, D, *bounds, scale), empty=empty, bytes=n[0].value,
+                           backward_bytes=n[1].value, qs=_strides(q), ks=_strides(k), vs=_strides(v),
+                           in_place=_in_place(q, False) and _in_place(k, False) and _in_place(v, False))
+
+
+def _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets):
+    """(plan, tensors, pointers of lengths and offsets): the tensors as the kernels can read them."""
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape,
+           v.stride(), v.dtype, v.get_device(), left, right, sinks, scale)
+    plan = _PLANS.get(key) or _plan(key, _window_plan, q, k, v, left, right, sinks, scale)
+    per_sequence = []
+    for t, name in ((lengths, "lengths"), (offsets, "offsets")):
+        if t is None:
+            per_sequence.append(None)
+            continue
+        if not torch.is_tensor(t) or t.dtype != torch.int32 or t.shape != q.shape[:1] or t.device != q.device:
+            _refuse(f"{name} must be an int32 tensor of one number per sequence, [{q.shape[0]}] on {q.device}")
+        per_sequence.append(t.contiguous())
+    if not plan.in_place or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _rows16(q, False), _rows16(k, False), _rows16(v, False)
+        plan = _window_plan(q, k, v, left, right, sinks, scale)
+    return plan, q, k, v, *per_sequence
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _device_error(ws, what):
+def _device_error(ws, stream, what):
     code = c_int32(0)
-    check(lib().solb200_read_device_error(ws.data_ptr(), ctypes.byref(code), _stream_ptr(ws.device)), what)
+    check(lib().solb200_read_device_error(ws.data_ptr(), ctypes.byref(code), stream), what)
 
 
 def _window_forward(q, k, v, left, right, sinks, scale, lengths, offsets, want_lse):
-    bounds, scale, lengths, offsets = _window_check(q, k, v, left, right, sinks, scale, lengths, offsets)
-    B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1:3]
-    if not (q.numel() and k.numel()):      # no queries, or no keys for them to see
-        out = torch.zeros((B, Tq, H, D), dtype=q.dtype, device=q.device)
-        return out, torch.full((B, H, Tq), -torch.inf, device=q.device) if want_lse else None
-    q, k, v = _rows16(q, False), _rows16(k, False), _rows16(v, False)
-    with _on(q.device):
-        out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
+    plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
+    B, Tq, _, H, _, D = plan.place[:6]
+    if plan.empty:      # no queries, or no keys for them to see
+        return (q.new_zeros((B, Tq, H, D)),
+                torch.full((B, H, Tq), -torch.inf, device=q.device) if want_lse else None)
+    index = q.get_device()
+    with _on(index):
+        out = q.new_empty((B, Tq, H, D))
         lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
-        n = _window_workspace(B, Tq, Tk, H, Hk, D, *bounds, 0)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        check(lib().solb200_window_attn(
-            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), out.data_ptr(),
-            _ptr(lse), _ptr(lengths), _ptr(offsets), B, Tq, Tk, H, Hk, D, *bounds, scale, ws.data_ptr(), n,
-            _stream_ptr(q.device)), "window_attn")
+        ws = torch.empty(plan.bytes, dtype=torch.uint8, device=q.device)
+        stream = _raw_stream(index)
+        rc = lib().solb200_window_attn(
+            q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, v.data_ptr(), plan.vs, out.data_ptr(), _ptr(lse),
+            _ptr(lengths), _ptr(offsets), *plan.place, ws.data_ptr(), plan.bytes, stream)
+        if rc:
+            check(rc, "window_attn")
         if _SYNC_CHECK:
-            _device_error(ws, "window_attn device error check")
+            _device_error(ws, stream, "window_attn device error check")
     return out, lse
 
 
@@ -265,30 +318,29 @@ def window_attn_backward(dout, q, k, v, out, lse, *, left=None, right=0, sinks=0
     """(dq, dk, dv) from the gradient of ``window_attn``'s output, its inputs, its output and
     its log-sum-exp (``return_lse``), with the same bounds. Sums are in a fixed order. ``q`` and
     ``dout`` have to be finite in every row, the rows of queries that see nothing included."""
-    bounds, scale, lengths, offsets = _window_check(q, k, v, left, right, sinks, scale, lengths, offsets)
-    B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1:3]
-    _bthd(dout, "dout", q.dtype, q.device, q.shape)
-    _bthd(out, "out", q.dtype, q.device, q.shape)
+    plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
+    B, Tq, Tk, H, Hk, D = plan.place[:6]
+    for t, name in ((dout, "dout"), (out, "out")):
+        if t.shape != q.shape or t.dtype != q.dtype or t.get_device() != q.get_device():
+            _bthd(t, name, q.dtype, q.device, q.shape)
     if lse.shape != (B, H, Tq) or lse.dtype != torch.float32 or lse.device != q.device:
         _refuse(f"lse must be float32 [{B}, {H}, {Tq}] on {q.device}")
-    if not (q.numel() and k.numel()):
-        return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    q, k, v, dout, out = (_rows16(t, False) for t in (q, k, v, dout, out))
-    lse = lse.contiguous()
-    with _on(q.device):
-        dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-        dk = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=q.device)
-        dv = torch.empty((B, Tk, Hk, D), dtype=q.dtype, device=q.device)
-        n = _window_workspace(B, Tq, Tk, H, Hk, D, *bounds, 1)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        check(lib().solb200_window_attn_backward(
-            dout.data_ptr(), _strides(dout), q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
-            _strides(v), out.data_ptr(), _strides(out), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            _ptr(lengths), _ptr(offsets), B, Tq, Tk, H, Hk, D, *bounds, scale, ws.data_ptr(), n,
-            _stream_ptr(q.device)), "window_attn_backward")
+    if plan.empty:
+        return tuple(t.new_zeros(t.shape) for t in (q, k, v))
+    dout, out, lse = _rows16(dout, False), _rows16(out, False), lse.contiguous()
+    index = q.get_device()
+    with _on(index):
+        dq, dk, dv = q.new_empty((B, Tq, H, D)), q.new_empty((B, Tk, Hk, D)), q.new_empty((B, Tk, Hk, D))
+        ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=q.device)
+        stream = _raw_stream(index)
+        rc = lib().solb200_window_attn_backward(
+            dout.data_ptr(), _strides(dout), q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, v.data_ptr(), plan.vs,
+            out.data_ptr(), _strides(out), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            _ptr(lengths), _ptr(offsets), *plan.place, ws.data_ptr(), plan.backward_bytes, stream)
+        if rc:
+            check(rc, "window_attn_backward")
         if _SYNC_CHECK:
-            _device_error(ws, "window_attn_backward device error check")
+            _device_error(ws, stream, "window_attn_backward device error check")
     return dq, dk, dv
 
 

@@ -209,6 +209,24 @@ def test_what_lies_behind_a_length_is_not_used(cuda_device, Tq):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("Tq", [1, 20])
+def test_keys_outside_every_window_are_not_used(cuda_device, Tq):
+    """NaN and infinities in keys between the sinks and the window, which no query sees, next to
+    keys that are seen, in the same tiles."""
+    q, k, v = (t.cuda() for t in _inputs(2, Tq, 700, 4, 2, 64, seed=12))
+    how = dict(left=100, sinks=5)
+    clean = solb200.window_attn(q, k, v, return_lse=True, **how)
+    dout = torch.randn_like(q)
+    grads = solb200.window_attn_backward(dout, q, k, v, *clean, **how)
+    k2, v2 = k.clone(), v.clone()
+    hidden = slice(5, 700 - Tq - 100)
+    k2[:, hidden], v2[:, hidden] = float("nan"), float("-inf")
+    dirty = solb200.window_attn(q, k2, v2, return_lse=True, **how)
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for a, b in zip(grads, solb200.window_attn_backward(dout, q, k2, v2, *dirty, **how)):
+        assert torch.equal(a, b)
+
+
 def test_agrees_with_the_dense_kernel(cuda_device):
     """No bounds: the dense call's attention, up to both calls' roundings."""
     q, k, v = _inputs(1, 500, 900, 3, 3, 128, seed=3)
