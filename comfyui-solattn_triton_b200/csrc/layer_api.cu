@@ -89,17 +89,26 @@ int32_t rope_params(RopeParams& p, const void* q, const int64_t* qs, const void*
 constexpr int kSlots = 148 * 2;   // forward CTAs resident on the GPU
 constexpr int kStepKeys = 64, kTileRows = 128;
 
-// Parts of the key axis. Alone, a tile's CTA takes one slot of the GPU for `steps` steps (the
-// most that the shapes and bounds allow; lengths live on the device) plus about kOpen steps'
-// time to open and close; parts make waves shorter where tiles are few, at the price of their
-// opening and of the joining kernel (kJoin steps' time). The cheapest count by that estimate.
-int window_splits(int64_t tiles, int64_t steps) {
-  constexpr int64_t kOpen = 3, kJoin = 6, kMostSplits = 64;
+// Parts of the key axis: the count with the least estimated time, in steps of 64 keys of one CTA
+// (about a microsecond, whether the tensor cores or memory set the pace). The CTAs run in waves
+// of kSlots, each wave as long as a part of `steps` steps (the most that the shapes and bounds allow;
+// lengths live on the device) but together no shorter than the GPU needs at nine tenths of its slots,
+// and kOpen steps to open and close each; the joining kernel takes kJoin and reads what the parts
+// wrote (`row_bytes` each, there and back at 5 MB a step), a third of a step per part.
+// Measured (us): 8 tiles x 64 steps 53 whole, 17.6 in 9 parts, 26.9 in 60; 40 tiles x 4096
+// steps 2841 whole, 755 in 7, 946 in 9 (two waves), 784 in 22; 520 tiles x 195 steps 451 whole, 479 in 2.
+int window_splits(int64_t tiles, int64_t steps, int64_t row_bytes) {
+  constexpr double kOpen = 3, kJoin = 2;
+  constexpr int kMostSplits = 64;
+  const double whole = (double)tiles * steps / (0.9 * kSlots);
   int best = 1;
-  int64_t best_cost = (tiles + kSlots - 1) / kSlots * (steps + kOpen);
-  for (int n = 2; n <= kMostSplits && n * 2 <= steps; ++n) {
-    const int64_t cost = (tiles * n + kSlots - 1) / kSlots * ((steps + n - 1) / n + kOpen) + kJoin;
-    if (cost < best_cost) {
+  double best_cost = 0;
+  for (int n = 1; n <= kMostSplits && (n == 1 || n * 2 <= steps); ++n) {
+    const int64_t waves = (tiles * n + kSlots - 1) / kSlots;
+    const double run = (double)waves * ((steps + n - 1) / n);
+    const double cost = (run > whole ? run : whole) + waves * kOpen +
+                        (n > 1 ? kJoin + n * (0.33 + 2.0 * row_bytes / 5e6) : 0);
+    if (n == 1 || cost < best_cost) {
       best_cost = cost;
       best = n;
     }
@@ -138,7 +147,7 @@ int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, in
     const int64_t span = p.sinks + left + right + (Tq < p.TPT ? Tq : p.TPT);
     if (span < keys) keys = span;
   }
-  p.nsplit = window_splits(tiles, (keys + kStepKeys - 1) / kStepKeys + 1);
+  p.nsplit = window_splits(tiles, (keys + kStepKeys - 1) / kStepKeys + 1, B * Tq * H * (D * 4 + 8));
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t cur = 256;   // the error word
   w.off_ml = cur;
@@ -311,9 +320,11 @@ int32_t solb200_window_attn_backward(const void* dout, const int64_t* dout_strid
     return rc;
   WinParams& p = w.p;
   if ((rc = bthd_map(&m.dout, dout, head_dim, heads, q_tokens, batch, dout_strides, p.G, p.TPT, "dout"))) return rc;
-  p.out = static_cast<__nv_bfloat16*>(dq);
-  p.dk = static_cast<__nv_bfloat16*>(dk);
-  p.dv = static_cast<__nv_bfloat16*>(dv);
+  const int64_t D = head_dim, dqs[3] = {q_tokens * heads * D, heads * D, D};
+  const int64_t dks[3] = {kv_tokens * kv_heads * D, kv_heads * D, D};
+  if ((rc = bthd_map(&m.o, dq, D, heads, q_tokens, batch, dqs, p.G, p.TPT, "dq"))) return rc;
+  if ((rc = bthd_map(&m.dk, dk, D, kv_heads, kv_tokens, batch, dks, 1, kTileRows, "dk"))) return rc;
+  if ((rc = bthd_map(&m.dv, dv, D, kv_heads, kv_tokens, batch, dks, 1, kTileRows, "dv"))) return rc;
   p.lse_in = lse;
   p.o_in = static_cast<const __nv_bfloat16*>(out);
   p.do_in = static_cast<const __nv_bfloat16*>(dout);

@@ -23,7 +23,7 @@ struct WinParams {
   float scale, s2;          // softmax scale, and times log2(e)
   int* err;
   uint64_t wait_ns;
-  __nv_bfloat16* out;       // forward: dense [B, Tq, H, D]
+  __nv_bfloat16* out;       // split forward: dense [B, Tq, H, D]
   float* lse;               // forward: [B, H, Tq] or null
   float* part_o;            // split forward: [nsplit, B, Tq, H, D] unnormalised sums
   float2* part_ml;          // split forward: [nsplit, B, Tq, H] (row maximum in log2 units, row sum)
@@ -33,7 +33,6 @@ struct WinParams {
   int64_t os[3], dos[3];    // strides {batch, token, head}
   float* rows_lse;          // [B, Hk, nqt, 128] lse * log2(e) by tile row (+inf: nothing seen, or no row)
   float* rows_delta;        // [B, Hk, nqt, 128] sum(dO * O) by tile row
-  __nv_bfloat16 *dk, *dv;
   int nkt;                  // key tiles of 128
 };
 
@@ -109,7 +108,8 @@ struct WinUnseen {
 };
 
 struct WinMaps {
-  CUtensorMap q, k, v, o, dout;
+  CUtensorMap q, k, v, o;        // o: the forward's output, the gradient's dq
+  CUtensorMap dout, dk, dv;      // gradient
 };
 
 cudaError_t launch_window_fwd(int hd, const WinMaps& m, const WinParams& p, cudaStream_t st);

@@ -32,6 +32,7 @@ constexpr int kTile = 128;
 constexpr uint32_t kBox = kTile * 128;   // a 128-row box of 64 bf16 columns
 constexpr int kSoftmax = 512;            // softmax threads: 4 per TMEM lane, 32 columns each
 constexpr int kThreads = kSoftmax + 64;
+constexpr int kPolyShare = 8;            // of a thread's 8 groups of 4 exponentials, those with 2 on the FMA pipe
 constexpr int kFewSteps = 3;             // query tiles with up to this many key steps refine delta
 
 // D (128 x 128) = A B^T, both K-major in shared memory (HD columns).
@@ -45,16 +46,16 @@ __device__ __forceinline__ void mma_scores(uint32_t mine, uint32_t d, uint64_t a
   }
 }
 
-// D (128 x HD) += A B, A bf16 in TMEM (32 of the 128 summed rows at a, a + 32, a + 64, a + 96,
-// each in the columns that its softmax threads read the scores from), B MN-major in shared memory
-// (128 rows of HD columns).
+// D (128 x HD) += A B over a quarter of the 128 summed rows, those of one column group: A bf16 in
+// TMEM (at a + 32 quarter, in the columns that the group's threads read the scores from), B
+// MN-major in shared memory (128 rows of HD columns).
 template <int HD>
-__device__ __forceinline__ void mma_sum(uint32_t mine, uint32_t d, uint32_t a, uint64_t b, bool first) {
+__device__ __forceinline__ void mma_sum_quarter(uint32_t mine, uint32_t d, uint32_t a, uint64_t b, int quarter, bool first) {
   constexpr uint32_t IDESC = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 1, 128, HD);
 #pragma unroll
-  for (int k = 0; k < kTile / 16; ++k)
-    mma_bf16_ts_warp(mine, d, a + (k >> 1) * 32 + (k & 1) * 8, desc_at(b, k * 2048), IDESC,
-                     (first && k == 0) ? 0u : 1u);
+  for (int k = 0; k < 2; ++k)
+    mma_bf16_ts_warp(mine, d, a + quarter * 32 + k * 8, desc_at(b, (quarter * 2 + k) * 2048), IDESC,
+                     (first && quarter == 0 && k == 0) ? 0u : 1u);
 }
 
 // Descriptors of a tile of 128 rows x HD columns: as a K-major operand (rows are M or N), and as
@@ -70,26 +71,28 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int i0, int 
     *reinterpret_cast<uint4*>(tile + (i / per) * kBox + first * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// A row of the scaled accumulator, columns [c0, c0 + NC), as bf16 to global memory.
+// Channels [c0, c0 + NC) of a lane's row of the scaled accumulator, as bf16 into a tile of 128-row
+// boxes with the 128-byte swizzle of a TMA store. (Rows stored from the lanes straight to global
+// memory cost about 7000 cycles a tile: 16 bytes from each of 32 rows per instruction.)
 template <int NC>
-__device__ __forceinline__ void store_row(uint32_t taddr, float scale, __nv_bfloat16* dst, bool live, bool zero) {
+__device__ __forceinline__ void stage_row(uint32_t taddr, float scale, uint8_t* tile, int row, int c0, bool zero) {
 #pragma unroll 1
-  for (int c = 0; c < NC / 32; ++c) {
+  for (int c = c0; c < c0 + NC; c += 32) {
     uint32_t r[32];
     if (!zero) {
-      tmem_ld32(taddr + c * 32, r);
+      tmem_ld32(taddr + c, r);
       tmem_wait_ld();
     }
-    if (live) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        uint32_t w[4];
+    for (int v = 0; v < 4; ++v) {
+      uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = zero ? 0u : pack_bf16x2(__uint_as_float(r[v * 8 + 2 * i]) * scale,
-                                         __uint_as_float(r[v * 8 + 2 * i + 1]) * scale);
-        *reinterpret_cast<uint4*>(dst + c * 32 + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int i = 0; i < 4; ++i)
+        w[i] = zero ? 0u : pack_bf16x2(__uint_as_float(r[v * 8 + 2 * i]) * scale,
+                                       __uint_as_float(r[v * 8 + 2 * i + 1]) * scale);
+      const int chunk = ((c & 63) >> 3) + v;
+      *reinterpret_cast<uint4*>(tile + (c >> 6) * kBox + row * 128 + ((chunk ^ (row & 7)) << 4)) =
+          make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
 }
 
 // 32 columns of P for one TMEM lane: 2^(s * s2 - lse * log2(e)). `nl(i)` gives -lse * log2(e) of
-// columns i and i + 1 (where a lane is a query row, the same for all).
+// columns 4 i .. 4 i + 3 (where a lane is a query row, the same for all).
 template <bool MASKED, typename NL>
 __device__ __forceinline__ void probs(uint32_t t_s, float s2, uint32_t mask, float2 (&pr)[16], NL&& nl) {
   uint32_t r[32];
@@ -139,12 +142,18 @@ __device__ __forceinline__ void probs(uint32_t t_s, float s2, uint32_t mask, flo
   tmem_wait_ld();
   const float2 s22 = make_float2(s2, s2);
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), s22, nl(i));
-    pr[i / 2] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-    if (MASKED) {
-      if (!((mask >> i) & 1u)) pr[i / 2].x = 0.f;
-      if (!((mask >> (i + 1)) & 1u)) pr[i / 2].y = 0.f;
+  for (int i = 0; i < 8; ++i) {
+    const float4 l = nl(i);
+    const float2 x = fma2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), s22, make_float2(l.x, l.y));
+    const float2 y = fma2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), s22, make_float2(l.z, l.w));
+    pr[2 * i] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+    pr[2 * i + 1] = kPolyShare > i ? exp2_poly2(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+  }
+  if (MASKED) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (!((mask >> (2 * i)) & 1u)) pr[i].x = 0.f;
+      if (!((mask >> (2 * i + 1)) & 1u)) pr[i].y = 0.f;
     }
   }
 }
@@ -173,6 +182,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                  const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                   const __grid_constant__ WinParams p) {
   pdl_begin();
   constexpr int NBOX = HD / 64;
@@ -192,11 +202,11 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* bar_dv = bars + 5;           // [2] dV(i) complete
   uint64_t* bar_dk = bars + 7;           // [2] dK(i) complete
   uint64_t* bar_s = bars + 9;
-  uint64_t* bar_p = bars + 10;
-  uint64_t* bar_dp = bars + 11;
-  uint64_t* bar_ds = bars + 12;
-  uint64_t* bar_drain = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint64_t* bar_dp = bars + 10;
+  uint64_t* bar_drain = bars + 11;
+  uint64_t* bar_p = bars + 12;           // [4] by column group
+  uint64_t* bar_ds = bars + 16;          // [4]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
@@ -221,10 +231,12 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(bar_dv + i, 1);
       mbar_init(bar_dk + i, 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar_p + i, kSoftmax / 4);
+      mbar_init(bar_ds + i, kSoftmax / 4);
+    }
     mbar_init(bar_s, 1);
-    mbar_init(bar_p, kSoftmax);
     mbar_init(bar_dp, 1);
-    mbar_init(bar_ds, kSoftmax);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
@@ -313,8 +325,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int i = 0; ok && i < n; ++i) {
         const int st = i & 1, nx = st ^ 1;
         const uint32_t par = (i >> 1) & 1, npar = ((i + 1) >> 1) & 1;
-        if (!(ok = wait(bar_p, i & 1))) break;
-        mma_sum<HD>(mine, tDV, tS, desc_at(g_sum, st * TILE), i == 0);
+        for (int c = 0; ok && c < 4; ++c)
+          if ((ok = wait(bar_p + c, i & 1))) mma_sum_quarter<HD>(mine, tDV, tS, desc_at(g_sum, st * TILE), c, i == 0);
+        if (!ok) break;
         tc_commit_warp(mine, bar_dv + st);
         if (i + 1 < n) {
           // S(i+1) overwrites P(i): dV(i) has to have read it
@@ -322,8 +335,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, nx * TILE));
           tc_commit_warp(mine, bar_s);
         }
-        if (!(ok = wait(bar_ds, i & 1))) break;
-        mma_sum<HD>(mine, tDK, tDP, desc_at(q_sum, st * TILE), i == 0);
+        for (int c = 0; ok && c < 4; ++c)
+          if ((ok = wait(bar_ds + c, i & 1))) mma_sum_quarter<HD>(mine, tDK, tDP, desc_at(q_sum, st * TILE), c, i == 0);
+        if (!ok) break;
         tc_commit_warp(mine, bar_dk + st);
         if (i + 1 < n) {
           if (!(ok = wait(bar_g + nx, npar) && wait(bar_dk + st, par))) break;
@@ -345,8 +359,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, t0 = (q_begin + i) * p.TPT;
       const int64_t pa = seq.off + t0, pb = pa + p.TPT - 1;
-      const float2* neg = reinterpret_cast<const float2*>(sRow + st * 256 + c0);
-      const float2* ndelta = neg + 64;
+      const float4* neg = reinterpret_cast<const float4*>(sRow + st * 256 + c0);
+      const float4* ndelta = neg + 32;
       // every query of the tile sees every key of the tile?
       const bool full = j0 + kTile <= seq.L && (p.right < 0 || pa + p.right >= j0 + kTile - 1) &&
                         (p.left < 0 || pb - p.left <= j0 || j0 + kTile <= p.sinks);
@@ -360,31 +374,44 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!(ok = mbar_wait_warp(bar_s, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
       float2 pr[16], dp[16];
-      if (full) probs<false>(ts, p.s2, mask, pr, [&](int c) { return neg[c / 2]; });
-      else probs<true>(ts, p.s2, mask, pr, [&](int c) { return neg[c / 2]; });
+      if (full) probs<false>(ts, p.s2, mask, pr, [&](int c) { return neg[c]; });
+      else probs<true>(ts, p.s2, mask, pr, [&](int c) { return neg[c]; });
       store_cols(ts, pr);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(bar_p);
+      mbar_arrive(bar_p + wg);
       if (!(ok = mbar_wait_warp(bar_dp, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
       if (full) load_dp<false>(tdp, mask, dp);
       else load_dp<true>(tdp, mask, dp);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) dp[c] = mul2(pr[c], add2(dp[c], ndelta[c]));
+      for (int c = 0; c < 8; ++c) {
+        const float4 d = ndelta[c];
+        dp[2 * c] = mul2(pr[2 * c], add2(dp[2 * c], make_float2(d.x, d.y)));
+        dp[2 * c + 1] = mul2(pr[2 * c + 1], add2(dp[2 * c + 1], make_float2(d.z, d.w)));
+      }
       store_cols(tdp, dp);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(bar_ds);
+      mbar_arrive(bar_ds + wg);
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok) {
-      // two of the four column groups store dV, two dK, half of the channels each
+      // two of the four column groups take dV, two dK, half of the channels each; the tiles of V and
+      // K are free (every product is complete)
       constexpr int NC = HD / 2;
-      const int half = (wg & 1) * NC;
-      __nv_bfloat16* dst = (wg < 2 ? p.dv : p.dk) + (((int64_t)b * p.Tk + j) * p.Hk + hk) * HD + half;
-      store_row<NC>((wg < 2 ? tDV : tDK) + lane_base + half, wg < 2 ? 1.f : p.scale, dst, j < p.Tk, n == 0);
+      stage_row<NC>((wg < 2 ? tDV : tDK) + lane_base, wg < 2 ? 1.f : p.scale, wg < 2 ? sV : sK, row, (wg & 1) * NC,
+                    n == 0);
+      fence_proxy_async_smem();
+    }
+    if (named_bar_all(1, kSoftmax, ok) && threadIdx.x == 0) {
+      for (int i = 0; i < NBOX; ++i) {
+        tma_store_4d(&tm_dv, sV + i * kBox, i * 64, hk, j0, b);
+        tma_store_4d(&tm_dk, sK + i * kBox, i * 64, hk, j0, b);
+      }
+      bulk_commit_group();
+      bulk_wait_group_read0();
     }
   }
   tc_fence_before();
@@ -399,7 +426,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                 const __grid_constant__ WinParams p) {
+                 const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ WinParams p) {
   pdl_begin();
   constexpr int NBOX = HD / 64;
   constexpr uint32_t TILE = NBOX * kBox;
@@ -417,9 +444,9 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* bar_dq = bars + 6;           // [3] dQ(i) complete
   uint64_t* bar_dp = bars + 9;           // [2]
   uint64_t* bar_s = bars + 11;           // [2]
-  uint64_t* bar_ds = bars + 13;
-  uint64_t* bar_drain = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* bar_ds = bars + 13;          // [4] by column group
+  uint64_t* bar_drain = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int id = blockIdx.x;
@@ -449,7 +476,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(bar_dp + i, 1);
       mbar_init(bar_s + i, 1);
     }
-    mbar_init(bar_ds, kSoftmax);
+    for (int i = 0; i < 4; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
@@ -511,7 +538,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
   } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
-    //   S(0) dP(0) S(1) | dP(i+1) dQ(i) S(i+2) | ...
+    //   S(0) dP(0) S(1) | dQ(i) dP(i+1) S(i+2) | ...
     if (n > 0) {
       const uint32_t mine = elect_one();
       const uint64_t q_rows = rows_desc(sQ), g_rows = rows_desc(sG), k_rows = rows_desc(sK), v_rows = rows_desc(sV);
@@ -535,10 +562,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       };
       bool ok = wait(bar_q, 0) && issue_s(0) && issue_dp(0) && (n == 1 || issue_s(1));
       for (int i = 0; ok && i < n; ++i) {
-        // (the softmax has taken dP(i) out)
-        if (!(ok = wait(bar_ds, i & 1) && (i + 1 >= n || issue_dp(i + 1)))) break;
-        if (i >= npre) mma_sum<HD>(mine, tDQ, tS + (i & 1) * 128, desc_at(k_sum, (i % 3) * TILE), i == npre);
+        for (int c = 0; ok && c < 4; ++c)
+          if ((ok = wait(bar_ds + c, i & 1)) && i >= npre)
+            mma_sum_quarter<HD>(mine, tDQ, tS + (i & 1) * 128, desc_at(k_sum, (i % 3) * TILE), c, i == npre);
+        if (!ok) break;
         tc_commit_warp(mine, bar_dq + i % 3);
+        // (every softmax thread has taken its dP(i) out)
+        if (i + 1 < n && !(ok = issue_dp(i + 1))) break;
         // S(i+2) overwrites dS(i): dQ(i) has to have read it
         if (i + 2 < n) ok = wait(bar_dq + i % 3, (i / 3) & 1) && issue_s(i + 2);
       }
@@ -581,8 +611,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       tc_fence_after();
       float2 pr[16], dp[16];
       if (ok) {
-        if (full) probs<false>(ts, p.s2, mask, pr, [&](int) { return make_float2(neg, neg); });
-        else probs<true>(ts, p.s2, mask, pr, [&](int) { return make_float2(neg, neg); });
+        if (full) probs<false>(ts, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
+        else probs<true>(ts, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
         ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
         tc_fence_after();
       }
@@ -618,13 +648,19 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_wait_st();
       }
       tc_fence_before();
-      mbar_arrive(bar_ds);
+      mbar_arrive(bar_ds + wg);
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok && wg < HD / 32) {
-      const int64_t orow = ((int64_t)b * p.Tq + t0 + tok) * p.H + hk * p.G + head;
-      store_row<32>(tDQ + lane_base + wg * 32, p.scale, p.out + orow * HD + wg * 32, live, n == 0);
+      // (the tile of Q is free: every product is complete)
+      stage_row<32>(tDQ + lane_base, p.scale, sQ, row, wg * 32, n == 0);
+      fence_proxy_async_smem();
+    }
+    if (named_bar_all(1, kSoftmax, ok) && threadIdx.x == 0) {
+      for (int i = 0; i < NBOX; ++i) tma_store_4d(&tm_dq, sQ + i * kBox, i * 64, hk * p.G, t0, b);
+      bulk_commit_group();
+      bulk_wait_group_read0();
     }
   }
   tc_fence_before();
@@ -638,7 +674,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 template <int HD>
 cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   constexpr size_t TILE = (HD / 64) * kBox;
-  constexpr size_t smem_kv = 6 * TILE + 2048 + 128 + 1024, smem_q = 7 * TILE + 128 + 1024;
+  constexpr size_t smem_kv = 6 * TILE + 2048 + 256 + 1024, smem_q = 7 * TILE + 256 + 1024;
   static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
   cudaError_t e = allow_smem(window_dkv_kernel<HD>, smem_kv, allowed_kv);
   if (e == cudaSuccess) e = allow_smem(window_dq_kernel<HD>, smem_q, allowed_q);
@@ -648,10 +684,10 @@ cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   // window_dq_kernel leaves refined deltas for window_dkv_kernel
   e = launch_pdl(window_dq_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nqt)), dim3(kThreads), smem_q, st, m.q,
-                 m.k, m.v, m.dout, p);
+                 m.k, m.v, m.dout, m.o, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(window_dkv_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nkt)), dim3(kThreads), smem_kv, st,
-                    m.q, m.k, m.v, m.dout, p);
+                    m.q, m.k, m.v, m.dout, m.dk, m.dv, p);
 }
 
 }  // namespace

@@ -55,7 +55,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* bar_drain = bars + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // CTA -> (batch, key head, tile, part): a head's tiles together (they share K and V in
   // L2), the last tiles first (under a causal mask they see the most keys)
   int id = blockIdx.x;
@@ -69,7 +69,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kStep> steps(p, seq.L, pa, pb);
   const int s_begin = (int)((int64_t)steps.n * split / p.nsplit);
-  const int nsteps = (int)((int64_t)steps.n * (split + 1) / p.nsplit) - s_begin;
+  const int nsteps = __shfl_sync(0xffffffffu, (int)((int64_t)steps.n * (split + 1) / p.nsplit) - s_begin, 0);
   const int rows = ntok * p.G;                     // rows of this tile that exist
   const int active = (rows + 31) / 32;             // softmax warps that hold any
 
@@ -139,47 +139,47 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
   } else if (warp == 5) {
     // -------------------------------------------------------------- MMA issuer
-    if (lane == 0 && nsteps > 0) {
-      const uint32_t q_base = smem_u32(sQ), k_base = smem_u32(sK), v_base = smem_u32(sV);
+    if (nsteps > 0) {
+      const uint32_t mine = elect_one();
+      const uint64_t q_desc = make_sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = make_sw128_desc(smem_u32(sK), 16, 1024);
+      const uint64_t v_desc = make_sw128_desc(smem_u32(sV), HBOX, 1024);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool done = mbar_wait_warp(bar, parity, p.err, kErrWaitMma, p.wait_ns);
+        tc_fence_after();
+        return done;
+      };
       auto issue_qk = [&](int s) {
         const int slot = s & 1;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t qo = (k >> 2) * QBOX + (k & 3) * 32;
-          const uint32_t ko = slot * SLOT + (k >> 2) * HBOX + (k & 3) * 32;
-          mma_bf16_ss(tS + slot * 64, make_sw128_desc(q_base + qo, 16, 1024),
-                      make_sw128_desc(k_base + ko, 16, 1024), IDESC_QK, k > 0);
-        }
-        tc_commit(bar_sfull + slot);
+        for (int k = 0; k < HD / 16; ++k)
+          mma_bf16_ss_warp(mine, tS + slot * 64, desc_at(q_desc, (k >> 2) * QBOX + (k & 3) * 32),
+                           desc_at(k_desc, slot * SLOT + (k >> 2) * HBOX + (k & 3) * 32), IDESC_QK, k > 0);
+        tc_commit_warp(mine, bar_sfull + slot);
       };
-      bool ok = mbar_wait(bar_q, 0, p.err, kErrWaitMma, p.wait_ns);
+      bool ok = wait(bar_q, 0);
       for (int s = 0; ok && s < min(2, nsteps); ++s) {
-        if (!(ok = mbar_wait(bar_kfull + s, 0, p.err, kErrWaitMma, p.wait_ns))) break;
-        tc_fence_after();
+        if (!(ok = wait(bar_kfull + s, 0))) break;
         issue_qk(s);
       }
       for (int s = 0; ok && s < nsteps; ++s) {
         const int slot = s & 1;
         const uint32_t par = (s >> 1) & 1;
-        if (!(ok = mbar_wait(bar_pfull + slot, par, p.err, kErrWaitMma, p.wait_ns))) break;
-        if (!(ok = mbar_wait(bar_vfull + slot, par, p.err, kErrWaitMma, p.wait_ns))) break;
-        tc_fence_after();
+        if (!(ok = wait(bar_pfull + slot, par) && wait(bar_vfull + slot, par))) break;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_bf16_ts(tO, tS + slot * 64 + kk * 8, make_sw128_desc(v_base + slot * SLOT + kk * 2048, HBOX, 1024),
-                      IDESC_PV, (s > 0 || kk > 0) ? 1u : 0u);
-        tc_commit(bar_pvdone + slot);
+          mma_bf16_ts_warp(mine, tO, tS + slot * 64 + kk * 8, desc_at(v_desc, slot * SLOT + kk * 2048), IDESC_PV,
+                           (s > 0 || kk > 0) ? 1u : 0u);
+        tc_commit_warp(mine, bar_pvdone + slot);
         if (s + 2 < nsteps) {
           // QK(s+2) overwrites slot s's P: PV(s) has to have read it
-          if (!(ok = mbar_wait(bar_pvdone + slot, par, p.err, kErrWaitMma, p.wait_ns))) break;
-          if (!(ok = mbar_wait(bar_kfull + slot, ((s + 2) >> 1) & 1, p.err, kErrWaitMma, p.wait_ns))) break;
-          tc_fence_after();
+          if (!(ok = wait(bar_pvdone + slot, par) && wait(bar_kfull + slot, ((s + 2) >> 1) & 1))) break;
           issue_qk(s + 2);
         }
       }
-      // every MMA this thread issued has completed once bar_drain fires
-      tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, p.err, kErrWaitDrain);
+      // every product issued has completed once bar_drain fires
+      tc_commit_warp(mine, bar_drain);
+      mbar_wait_warp(bar_drain, 0, p.err, kErrWaitDrain);
     }
   } else {
     // ------------------------------------------------- softmax + epilogue (rows)
