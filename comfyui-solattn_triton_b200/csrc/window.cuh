@@ -79,11 +79,6 @@ struct WinSteps {
   __device__ int key0(int s) const { return (s < n1 ? s : start + s - n1) * STEP; }
 };
 
-// Whether every query at positions [pa, pb] sees all of the keys [k0, k0 + n).
-__device__ __forceinline__ bool win_full(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
-  return k0 + n <= win_hi(p, L, pa) && (k0 >= win_lo(p, pb) || k0 + n <= p.sinks);
-}
-
 __device__ __forceinline__ uint32_t win_low_bits(int n) {
   return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
 }

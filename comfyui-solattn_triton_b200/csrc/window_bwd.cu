@@ -7,7 +7,8 @@
 //   window_dkv_kernel  a tile of 128 keys; walks the query tiles that see any of them (all
 //                      query heads of the key head are stacked in a tile's rows, so shared
 //                      heads need no sum afterwards): S^T and dP^T in TMEM, one key per
-//                      lane; P^T and dS^T go back as bf16 A operands of dV += P^T dO, dK += dS^T Q;
+//                      lane; P^T and dS^T go back, both over dP^T, as bf16 A operands of
+//                      dV += P^T dO, dK += dS^T Q;
 //   window_dq_kernel   a tile of 128 query rows; walks the 128-key steps of WinSteps: S and
 //                      dP, one query row per lane; dQ += dS K.
 // All products are M = 128, N = 128 (N = head_dim for the sums); sums stay in 32 bits in TMEM,
@@ -32,7 +33,7 @@ constexpr int kTile = 128;
 constexpr uint32_t kBox = kTile * 128;   // a 128-row box of 64 bf16 columns
 constexpr int kSoftmax = 512;            // softmax threads: 4 per TMEM lane, 32 columns each
 constexpr int kThreads = kSoftmax + 64;
-constexpr int kPolyShare = 8;            // of a thread's 8 groups of 4 exponentials, those with 2 on the FMA pipe
+constexpr int kPolyShare = 0;            // of a thread's 8 groups of 4 exponentials, those with 2 on the FMA pipe
 constexpr int kFewSteps = 3;             // query tiles with up to this many key steps refine delta
 
 // D (128 x 128) = A B^T, both K-major in shared memory (HD columns).
@@ -47,8 +48,8 @@ __device__ __forceinline__ void mma_scores(uint32_t mine, uint32_t d, uint64_t a
 }
 
 // D (128 x HD) += A B over a quarter of the 128 summed rows, those of one column group: A bf16 in
-// TMEM (at a + 32 quarter, in the columns that the group's threads read the scores from), B
-// MN-major in shared memory (128 rows of HD columns).
+// TMEM (at a + 32 quarter, in columns that only the group's threads read and write), B MN-major in
+// shared memory (128 rows of HD columns).
 template <int HD>
 __device__ __forceinline__ void mma_sum_quarter(uint32_t mine, uint32_t d, uint32_t a, uint64_t b, int quarter, bool first) {
   constexpr uint32_t IDESC = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 1, 128, HD);
@@ -133,13 +134,10 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   }
 }
 
-// 32 columns of P for one TMEM lane: 2^(s * s2 - lse * log2(e)). `nl(i)` gives -lse * log2(e) of
-// columns 4 i .. 4 i + 3 (where a lane is a query row, the same for all).
+// 32 columns of P for one TMEM lane: 2^(s * s2 - lse * log2(e)), s the raw scores in r. `nl(i)` gives
+// -lse * log2(e) of columns 4 i .. 4 i + 3 (where a lane is a query row, the same for all).
 template <bool MASKED, typename NL>
-__device__ __forceinline__ void probs(uint32_t t_s, float s2, uint32_t mask, float2 (&pr)[16], NL&& nl) {
-  uint32_t r[32];
-  tmem_ld32(t_s, r);
-  tmem_wait_ld();
+__device__ __forceinline__ void probs(const uint32_t (&r)[32], float s2, uint32_t mask, float2 (&pr)[16], NL&& nl) {
   const float2 s22 = make_float2(s2, s2);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -199,14 +197,13 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* bar_kv = bars + 0;
   uint64_t* bar_q = bars + 1;            // [2] Q and its rows' numbers
   uint64_t* bar_g = bars + 3;            // [2] dO
-  uint64_t* bar_dv = bars + 5;           // [2] dV(i) complete
-  uint64_t* bar_dk = bars + 7;           // [2] dK(i) complete
-  uint64_t* bar_s = bars + 9;
-  uint64_t* bar_dp = bars + 10;
-  uint64_t* bar_drain = bars + 11;
-  uint64_t* bar_p = bars + 12;           // [4] by column group
-  uint64_t* bar_ds = bars + 16;          // [4]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* bar_done = bars + 5;         // [2] dV(i) and dK(i) complete
+  uint64_t* bar_s = bars + 7;
+  uint64_t* bar_taken = bars + 8;        // S(i) is in the softmax threads' registers
+  uint64_t* bar_dp = bars + 9;
+  uint64_t* bar_drain = bars + 10;
+  uint64_t* bar_ds = bars + 11;          // [4] P(i) and dS(i) stored, by column group
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
@@ -228,14 +225,11 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_q + i, 1);
       mbar_init(bar_g + i, 1);
-      mbar_init(bar_dv + i, 1);
-      mbar_init(bar_dk + i, 1);
+      mbar_init(bar_done + i, 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(bar_p + i, kSoftmax / 4);
-      mbar_init(bar_ds + i, kSoftmax / 4);
-    }
+    for (int i = 0; i < 4; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
     mbar_init(bar_s, 1);
+    mbar_init(bar_taken, kSoftmax);
     mbar_init(bar_dp, 1);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
@@ -287,10 +281,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       bool ok = true;
       for (int i = 2; i < n; ++i) {
-        if (!(ok = mbar_wait(bar_dv + (i & 1), ((i - 2) >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-        load_g(last_g = i);
-        if (!(ok = mbar_wait(bar_dk + (i & 1), ((i - 2) >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        if (!(ok = mbar_wait(bar_done + (i & 1), ((i - 2) >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
         load_q(last_q = i);
+        load_g(last_g = i);
       }
       if (!ok) {
         // exit path: every issued copy lands before the CTA's shared memory goes away
@@ -301,8 +294,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
   } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
-    //   S(0) dP(0) | dV(i) S(i+1) dK(i) dP(i+1) | ...  The softmax works on dS(i) while
-    //   dV(i) and S(i+1) run, and on P(i+1) while dK(i) and dP(i+1) run.
+    //   S(0) dP(0) S(1) | dV(i) dK(i) dP(i+1) S(i+2) | ...  The softmax forms P(i+1) while dV(i),
+    //   dK(i) and dP(i+1) run, and dS(i+1) while S(i+2) runs.
     if (n > 0) {
       const uint32_t mine = elect_one();
       const uint64_t k_rows = rows_desc(sK), v_rows = rows_desc(sV), q_rows = rows_desc(sQ), g_rows = rows_desc(sG);
@@ -312,38 +305,31 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_after();
         return done;
       };
-      bool ok = wait(bar_kv, 0) && wait(bar_q, 0);
-      if (ok) {
-        mma_scores<HD>(mine, tS, k_rows, q_rows);
+      auto issue_s = [&](int i) {
+        if (!wait(bar_q + (i & 1), (i >> 1) & 1)) return false;
+        mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, (i & 1) * TILE));
         tc_commit_warp(mine, bar_s);
-        ok = wait(bar_g, 0);
-      }
-      if (ok) {
-        mma_scores<HD>(mine, tDP, v_rows, g_rows);
+        return true;
+      };
+      auto issue_dp = [&](int i) {
+        if (!wait(bar_g + (i & 1), (i >> 1) & 1)) return false;
+        mma_scores<HD>(mine, tDP, v_rows, desc_at(g_rows, (i & 1) * TILE));
         tc_commit_warp(mine, bar_dp);
-      }
+        return true;
+      };
+      bool ok = wait(bar_kv, 0) && issue_s(0) && issue_dp(0) && (n == 1 || (wait(bar_taken, 0) && issue_s(1)));
       for (int i = 0; ok && i < n; ++i) {
-        const int st = i & 1, nx = st ^ 1;
-        const uint32_t par = (i >> 1) & 1, npar = ((i + 1) >> 1) & 1;
-        for (int c = 0; ok && c < 4; ++c)
-          if ((ok = wait(bar_p + c, i & 1))) mma_sum_quarter<HD>(mine, tDV, tS, desc_at(g_sum, st * TILE), c, i == 0);
-        if (!ok) break;
-        tc_commit_warp(mine, bar_dv + st);
-        if (i + 1 < n) {
-          // S(i+1) overwrites P(i): dV(i) has to have read it
-          if (!(ok = wait(bar_q + nx, npar) && wait(bar_dv + st, par))) break;
-          mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, nx * TILE));
-          tc_commit_warp(mine, bar_s);
+        const int st = i & 1;
+        for (int c = 0; ok && c < 4; ++c) {
+          if (!(ok = wait(bar_ds + c, i & 1))) break;
+          mma_sum_quarter<HD>(mine, tDV, tDP, desc_at(g_sum, st * TILE), c, i == 0);
+          mma_sum_quarter<HD>(mine, tDK, tDP + 16, desc_at(q_sum, st * TILE), c, i == 0);
         }
-        for (int c = 0; ok && c < 4; ++c)
-          if ((ok = wait(bar_ds + c, i & 1))) mma_sum_quarter<HD>(mine, tDK, tDP, desc_at(q_sum, st * TILE), c, i == 0);
         if (!ok) break;
-        tc_commit_warp(mine, bar_dk + st);
-        if (i + 1 < n) {
-          if (!(ok = wait(bar_g + nx, npar) && wait(bar_dk + st, par))) break;
-          mma_scores<HD>(mine, tDP, v_rows, desc_at(g_rows, nx * TILE));
-          tc_commit_warp(mine, bar_dp);
-        }
+        tc_commit_warp(mine, bar_done + st);
+        // dP(i+1) overwrites P(i) and dS(i), S(i+2) S(i+1)
+        if (i + 1 < n) ok = wait(bar_done + st, (i >> 1) & 1) && issue_dp(i + 1);
+        if (ok && i + 2 < n) ok = wait(bar_taken, (i + 1) & 1) && issue_s(i + 2);
       }
       // every product issued has completed once bar_drain fires
       tc_commit_warp(mine, bar_drain);
@@ -355,42 +341,47 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tS + lane_base + c0, tdp = tDP + lane_base + c0;
     const int j = j0 + row;
+    // tokens [first, last) see this lane's key; tokens [full_first, full_last) see every key of the tile
+    const int first = p.right < 0 ? 0 : clamp_to((int64_t)j - p.right - seq.off, 0, p.Tq);
+    const int last = j >= seq.L ? 0 : (p.left < 0 || j < p.sinks ? p.Tq : clamp_to((int64_t)j + p.left - seq.off + 1, 0, p.Tq));
+    const int full_first = p.right < 0 ? 0 : clamp_to((int64_t)j0 + kTile - 1 - p.right - seq.off, 0, p.Tq);
+    const int full_last = j0 + kTile > seq.L ? 0
+                          : (p.left < 0 || j0 + kTile <= p.sinks ? p.Tq : clamp_to((int64_t)j0 + p.left - seq.off + 1, 0, p.Tq));
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, t0 = (q_begin + i) * p.TPT;
-      const int64_t pa = seq.off + t0, pb = pa + p.TPT - 1;
       const float4* neg = reinterpret_cast<const float4*>(sRow + st * 256 + c0);
       const float4* ndelta = neg + 32;
-      // every query of the tile sees every key of the tile?
-      const bool full = j0 + kTile <= seq.L && (p.right < 0 || pa + p.right >= j0 + kTile - 1) &&
-                        (p.left < 0 || pb - p.left <= j0 || j0 + kTile <= p.sinks);
+      // (rows of tokens past the last have P = 0 without a mask)
+      const bool full = t0 >= full_first && min(t0 + p.TPT, p.Tq) <= full_last;
       uint32_t mask = 0;
-      if (!full && j < seq.L) {
-        const int lo = p.right < 0 ? 0 : clamp_to((int64_t)j - p.right - pa, 0, p.TPT) * p.G;
-        const int hi = (p.left < 0 || j < p.sinks) ? kTile : clamp_to((int64_t)j + p.left - pa + 1, 0, p.TPT) * p.G;
+      if (!full) {
+        const int lo = min(max(first - t0, 0), p.TPT) * p.G, hi = min(max(last - t0, 0), p.TPT) * p.G;
         mask = win_low_bits(hi - c0) & ~win_low_bits(lo - c0);
       }
       if (!(ok = mbar_wait_warp(bar_q + st, (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       if (!(ok = mbar_wait_warp(bar_s, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
-      float2 pr[16], dp[16];
-      if (full) probs<false>(ts, p.s2, mask, pr, [&](int c) { return neg[c]; });
-      else probs<true>(ts, p.s2, mask, pr, [&](int c) { return neg[c]; });
-      store_cols(ts, pr);
-      tmem_wait_st();
+      uint32_t r[32];
+      tmem_ld32(ts, r);
+      tmem_wait_ld();
       tc_fence_before();
-      mbar_arrive(bar_p + wg);
+      mbar_arrive(bar_taken);
+      float2 pr[16], dp[16];
+      if (full) probs<false>(r, p.s2, mask, pr, [&](int c) { return neg[c]; });
+      else probs<true>(r, p.s2, mask, pr, [&](int c) { return neg[c]; });
       if (!(ok = mbar_wait_warp(bar_dp, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
       if (full) load_dp<false>(tdp, mask, dp);
       else load_dp<true>(tdp, mask, dp);
+      store_cols(tdp, pr);
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const float4 d = ndelta[c];
         dp[2 * c] = mul2(pr[2 * c], add2(dp[2 * c], make_float2(d.x, d.y)));
         dp[2 * c + 1] = mul2(pr[2 * c + 1], add2(dp[2 * c + 1], make_float2(d.z, d.w)));
       }
-      store_cols(tdp, dp);
+      store_cols(tdp + 16, dp);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(bar_ds + wg);
@@ -444,9 +435,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* bar_dq = bars + 6;           // [3] dQ(i) complete
   uint64_t* bar_dp = bars + 9;           // [2]
   uint64_t* bar_s = bars + 11;           // [2]
-  uint64_t* bar_ds = bars + 13;          // [4] by column group
-  uint64_t* bar_drain = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t* bar_ds = bars + 13;          // [2][4] by step parity (dS(i+1) may be stored before dS(i) is waited
+                                         // for) and column group
+  uint64_t* bar_drain = bars + 21;
+  uint64_t* bar_taken = bars + 22;       // dP(i) is in the softmax threads' registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int id = blockIdx.x;
@@ -476,7 +469,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(bar_dp + i, 1);
       mbar_init(bar_s + i, 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
+    for (int i = 0; i < 8; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
+    mbar_init(bar_taken, kSoftmax);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
@@ -538,7 +532,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
   } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
-    //   S(0) dP(0) S(1) | dQ(i) dP(i+1) S(i+2) | ...
+    //   S(0) dP(0) S(1) | dP(i+1) dQ(i) S(i+2) | ...
     if (n > 0) {
       const uint32_t mine = elect_one();
       const uint64_t q_rows = rows_desc(sQ), g_rows = rows_desc(sG), k_rows = rows_desc(sK), v_rows = rows_desc(sV);
@@ -562,13 +556,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       };
       bool ok = wait(bar_q, 0) && issue_s(0) && issue_dp(0) && (n == 1 || issue_s(1));
       for (int i = 0; ok && i < n; ++i) {
+        if (i + 1 < n && !(ok = wait(bar_taken, i & 1) && issue_dp(i + 1))) break;
         for (int c = 0; ok && c < 4; ++c)
-          if ((ok = wait(bar_ds + c, i & 1)) && i >= npre)
+          if ((ok = wait(bar_ds + (i & 1) * 4 + c, (i >> 1) & 1)) && i >= npre)
             mma_sum_quarter<HD>(mine, tDQ, tS + (i & 1) * 128, desc_at(k_sum, (i % 3) * TILE), c, i == npre);
         if (!ok) break;
         tc_commit_warp(mine, bar_dq + i % 3);
-        // (every softmax thread has taken its dP(i) out)
-        if (i + 1 < n && !(ok = issue_dp(i + 1))) break;
         // S(i+2) overwrites dS(i): dQ(i) has to have read it
         if (i + 2 < n) ok = wait(bar_dq + i % 3, (i / 3) & 1) && issue_s(i + 2);
       }
@@ -583,6 +576,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const bool live = row < rows;
     const int64_t pos = pa + tok;
     const int hi = live ? win_hi(p, seq.L, pos) : 0, lo = live ? win_lo(p, pos) : 0;
+    // every row of the tile sees the keys [full_lo, full_hi), and the sinks before full_hi
+    const int full_hi = win_hi(p, seq.L, pa), full_lo = win_lo(p, pb);
     const int64_t slot = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile + row;
     const float neg = p.rows_lse[slot];
     float ndelta = p.rows_delta[slot];
@@ -605,20 +600,25 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     for (int i = 0; i < n; ++i) {
       const int k0 = key0(i);
       const uint32_t ts = tS + (i & 1) * 128 + lane_base + c0, tdp = tDP + lane_base + c0;
-      const bool full = win_full(p, seq.L, pa, pb, k0, kTile);
+      const bool full = k0 + kTile <= full_hi && (k0 >= full_lo || k0 + kTile <= p.sinks);
       const uint32_t mask = !full && live ? win_bits(k0 + c0, lo, hi, p.sinks) : 0u;
       ok = mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
       tc_fence_after();
       float2 pr[16], dp[16];
       if (ok) {
-        if (full) probs<false>(ts, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
-        else probs<true>(ts, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
+        uint32_t r[32];
+        tmem_ld32(ts, r);
+        tmem_wait_ld();
+        if (full) probs<false>(r, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
+        else probs<true>(r, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
         ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
         tc_fence_after();
       }
       if (ok) {
         if (full) load_dp<false>(tdp, mask, dp);
         else load_dp<true>(tdp, mask, dp);
+        tc_fence_before();
+        mbar_arrive(bar_taken);
       }
       if (few) {
         if (ok && (i < npre || n == 1))
@@ -637,9 +637,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (!full && unseen.any(kTile)) {
           // (S(i) is complete, and bar_k was waited for before it was issued)
           if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+          // each column group zeroes the rows of its own quarter of the sum: bar_ds is per group
           uint8_t* tile = sK + (i % 3) * TILE;
-          for (int c = threadIdx.x; c < kTile * NBOX * 8; c += kSoftmax) {
-            const int r = c / (NBOX * 8), x = c % (NBOX * 8);
+          for (int c = threadIdx.x & 127; c < 32 * NBOX * 8; c += 128) {
+            const int r = c0 + c / (NBOX * 8), x = c % (NBOX * 8);
             if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
               *reinterpret_cast<uint4*>(tile + (x >> 3) * kBox + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
@@ -648,7 +649,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_wait_st();
       }
       tc_fence_before();
-      mbar_arrive(bar_ds + wg);
+      mbar_arrive(bar_ds + (i & 1) * 4 + wg);
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();

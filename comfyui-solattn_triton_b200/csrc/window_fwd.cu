@@ -189,6 +189,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const bool live = row < rows;
     const int64_t pos = pa + tok;
     const int hi = live ? win_hi(p, seq.L, pos) : 0, lo = live ? win_lo(p, pos) : 0;
+    // every row of the tile sees the keys [full_lo, full_hi), and the sinks before full_hi
+    const int full_hi = win_hi(p, seq.L, pa), full_lo = win_lo(p, pb);
     float m_ref = -INFINITY, l_sum = 0.f;
     bool ok = true;
     if (warp < active) {
@@ -203,7 +205,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tc_fence_after();
         };
         uint32_t bits[2];
-        if (win_full(p, seq.L, pa, pb, k0, kStep)) {
+        if (k0 + kStep <= full_hi && (k0 >= full_lo || k0 + kStep <= p.sinks)) {
           softmax_half<false, false, HD>(ts, tO + lane_base, bits, p.s2, m_ref, l_sum, s > 0, -1, 0.f, 1.f, drain);
         } else {
           bits[0] = live ? win_bits(k0, lo, hi, p.sinks) : 0u;
