@@ -477,27 +477,6 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&r);
 }
 
-// 2^x of a pair on the FMA and ALU pipes, for kernels whose special-function unit is the longest
-// queue: x = n + f with n the nearest integer (by adding 1.5 * 2^23), 2^f as a polynomial on
-// [-1/2, 1/2], and n added to the exponent bits. The coefficients are the minimax solution of
-// relative error with a constant term of 1, computed for this file by linear programming over
-// 4001 Chebyshev points: 2.9e-6 in fp32. x below -127 gives 0; x has to stay below 127; a NaN gives no
-// finite value.
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
-  const float2 big = make_float2(12582912.f, 12582912.f), neg_big = make_float2(-12582912.f, -12582912.f);
-  const float2 t = add2(x, big);
-  const float2 f = fma2(add2(t, neg_big), make_float2(-1.f, -1.f), x);
-  float2 y = make_float2(0.009585382416844368f, 0.009585382416844368f);
-  y = fma2(y, f, make_float2(0.05590662732720375f, 0.05590662732720375f));
-  y = fma2(y, f, make_float2(0.24024038016796112f, 0.24024038016796112f));
-  y = fma2(y, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
-  y = fma2(y, f, make_float2(1.f, 1.f));
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
-
 // add with rounding toward zero, two lanes at once
 __device__ __forceinline__ float2 add_rz2(float2 a, float2 b) {
   uint64_t r;

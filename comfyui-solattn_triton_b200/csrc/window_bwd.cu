@@ -33,7 +33,6 @@ constexpr int kTile = 128;
 constexpr uint32_t kBox = kTile * 128;   // a 128-row box of 64 bf16 columns
 constexpr int kSoftmax = 512;            // softmax threads: 4 per TMEM lane, 32 columns each
 constexpr int kThreads = kSoftmax + 64;
-constexpr int kPolyShare = 0;            // of a thread's 8 groups of 4 exponentials, those with 2 on the FMA pipe
 constexpr int kFewSteps = 3;             // query tiles with up to this many key steps refine delta
 
 // D (128 x 128) = A B^T, both K-major in shared memory (HD columns).
@@ -145,7 +144,7 @@ __device__ __forceinline__ void probs(const uint32_t (&r)[32], float s2, uint32_
     const float2 x = fma2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), s22, make_float2(l.x, l.y));
     const float2 y = fma2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), s22, make_float2(l.z, l.w));
     pr[2 * i] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-    pr[2 * i + 1] = kPolyShare > i ? exp2_poly2(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+    pr[2 * i + 1] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
   }
   if (MASKED) {
 #pragma unroll
@@ -187,23 +186,30 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   constexpr uint32_t TILE = NBOX * kBox;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  // (227 KB leave 768 bytes for the alignment of a base that is aligned already; one that needs
+  // more is refused)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (smem - smem_raw > 768) {
+    if (threadIdx.x == 0) atomicOr(p.err, kErrWaitLoad);
+    return;
+  }
   uint8_t* sK = smem;
   uint8_t* sV = sK + TILE;
-  uint8_t* sQ = sV + TILE;               // 2 stages
-  uint8_t* sG = sQ + 2 * TILE;           // dO, 2 stages
+  uint8_t* sQ = sV + TILE;               // 3 stages: Q(i) is read until dK(i), S(i+2) is next but one
+  uint8_t* sG = sQ + 3 * TILE;           // dO, 2 stages
   float* sRow = reinterpret_cast<float*>(sG + 2 * TILE);   // 2 stages of [-lse2 128, -delta 128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 256);
   uint64_t* bar_kv = bars + 0;
-  uint64_t* bar_q = bars + 1;            // [2] Q and its rows' numbers
-  uint64_t* bar_g = bars + 3;            // [2] dO
-  uint64_t* bar_done = bars + 5;         // [2] dV(i) and dK(i) complete
-  uint64_t* bar_s = bars + 7;
-  uint64_t* bar_taken = bars + 8;        // S(i) is in the softmax threads' registers
-  uint64_t* bar_dp = bars + 9;
-  uint64_t* bar_drain = bars + 10;
-  uint64_t* bar_ds = bars + 11;          // [4] P(i) and dS(i) stored, by column group
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* bar_q = bars + 1;            // [3]
+  uint64_t* bar_g = bars + 4;            // [2] dO and its rows' numbers
+  uint64_t* bar_done = bars + 6;         // [2] dV(i) and dK(i) complete
+  uint64_t* bar_s = bars + 8;
+  uint64_t* bar_taken = bars + 9;        // S(i) is in the softmax threads' registers
+  uint64_t* bar_dp = bars + 10;
+  uint64_t* bar_drain = bars + 11;
+  uint64_t* bar_p = bars + 12;           // [4] P(i) stored, by column group
+  uint64_t* bar_ds = bars + 16;          // [4] dS(i) stored
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
@@ -222,12 +228,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (threadIdx.x == 0) {
     mbar_init(bar_kv, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(bar_q + i, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_q + i, 1);
       mbar_init(bar_g + i, 1);
       mbar_init(bar_done + i, 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar_p + i, kSoftmax / 4);
+      mbar_init(bar_ds + i, kSoftmax / 4);
+    }
     mbar_init(bar_s, 1);
     mbar_init(bar_taken, kSoftmax);
     mbar_init(bar_dp, 1);
@@ -236,10 +245,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
   // rows that no box fills are summed over (with P = dS = 0): they have to be finite
   if (p.RT < kTile && n > 0)
-    for (int i = 0; i < 2; ++i) {
-      zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, kThreads);
-      zero_rows<HD>(sG + i * TILE, p.RT, threadIdx.x, kThreads);
-    }
+    for (int i = 0; i < 5; ++i) zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, kThreads);
   fence_proxy_async_smem();
   if (warp == kSoftmax / 32 + 1) {
     tmem_alloc(tmem_slot, 512);
@@ -257,19 +263,18 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_arrive_expect_tx(bar_kv, 2 * TILE);
       for (int i = 0; i < NBOX; ++i) tma_load_4d(sK + i * kBox, &tm_k, bar_kv, i * 64, hk, j0, b);
       auto load_q = [&](int i) {
-        const int st = i & 1, qt = q_begin + i;
-        mbar_arrive_expect_tx(bar_q + st, NBOX * p.RT * 128 + 1024);
+        mbar_arrive_expect_tx(bar_q + i % 3, NBOX * p.RT * 128);
         for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sQ + st * TILE + x * kBox, &tm_q, bar_q + st, x * 64, hk * p.G, qt * p.TPT, b);
-        const int64_t r = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile;
-        bulk_load(sRow + st * 256, p.rows_lse + r, 512, bar_q + st);
-        bulk_load(sRow + st * 256 + 128, p.rows_delta + r, 512, bar_q + st);
+          tma_load_4d(sQ + (i % 3) * TILE + x * kBox, &tm_q, bar_q + i % 3, x * 64, hk * p.G, (q_begin + i) * p.TPT, b);
       };
       auto load_g = [&](int i) {
-        const int st = i & 1;
-        mbar_arrive_expect_tx(bar_g + st, NBOX * p.RT * 128);
+        const int st = i & 1, qt = q_begin + i;
+        mbar_arrive_expect_tx(bar_g + st, NBOX * p.RT * 128 + 1024);
+        const int64_t r = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile;
+        bulk_load(sRow + st * 256, p.rows_lse + r, 512, bar_g + st);
+        bulk_load(sRow + st * 256 + 128, p.rows_delta + r, 512, bar_g + st);
         for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sG + st * TILE + x * kBox, &tm_do, bar_g + st, x * 64, hk * p.G, (q_begin + i) * p.TPT, b);
+          tma_load_4d(sG + st * TILE + x * kBox, &tm_do, bar_g + st, x * 64, hk * p.G, qt * p.TPT, b);
       };
       load_q(0);
       for (int i = 0; i < NBOX; ++i) tma_load_4d(sV + i * kBox, &tm_v, bar_kv, i * 64, hk, j0, b);
@@ -279,23 +284,24 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         load_q(last_q = 1);
         load_g(last_g = 1);
       }
+      if (n > 2) load_q(last_q = 2);
       bool ok = true;
-      for (int i = 2; i < n; ++i) {
-        if (!(ok = mbar_wait(bar_done + (i & 1), ((i - 2) >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-        load_q(last_q = i);
-        load_g(last_g = i);
+      for (int i = 0; i + 2 < n; ++i) {
+        if (!(ok = mbar_wait(bar_done + (i & 1), (i >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        load_g(last_g = i + 2);
+        if (i + 3 < n) load_q(last_q = i + 3);
       }
       if (!ok) {
         // exit path: every issued copy lands before the CTA's shared memory goes away
         mbar_wait(bar_kv, 0, p.err, kErrWaitDrain);
-        for (int i = max(0, last_q - 1); i <= last_q; ++i) mbar_wait(bar_q + (i & 1), (i >> 1) & 1, p.err, kErrWaitDrain);
+        for (int i = max(0, last_q - 2); i <= last_q; ++i) mbar_wait(bar_q + i % 3, (i / 3) & 1, p.err, kErrWaitDrain);
         for (int i = max(0, last_g - 1); i <= last_g; ++i) mbar_wait(bar_g + (i & 1), (i >> 1) & 1, p.err, kErrWaitDrain);
       }
     }
   } else if (warp == kSoftmax / 32 + 1) {
     // -------------------------------------------------------------- MMA issuer
     //   S(0) dP(0) S(1) | dV(i) dK(i) dP(i+1) S(i+2) | ...  The softmax forms P(i+1) while dV(i),
-    //   dK(i) and dP(i+1) run, and dS(i+1) while S(i+2) runs.
+    //   dK(i) and dP(i+1) run, and dS(i+1) while S(i+2) and dV(i+1) run.
     if (n > 0) {
       const uint32_t mine = elect_one();
       const uint64_t k_rows = rows_desc(sK), v_rows = rows_desc(sV), q_rows = rows_desc(sQ), g_rows = rows_desc(sG);
@@ -306,8 +312,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         return done;
       };
       auto issue_s = [&](int i) {
-        if (!wait(bar_q + (i & 1), (i >> 1) & 1)) return false;
-        mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, (i & 1) * TILE));
+        if (!wait(bar_q + i % 3, (i / 3) & 1)) return false;
+        mma_scores<HD>(mine, tS, k_rows, desc_at(q_rows, (i % 3) * TILE));
         tc_commit_warp(mine, bar_s);
         return true;
       };
@@ -320,11 +326,11 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       bool ok = wait(bar_kv, 0) && issue_s(0) && issue_dp(0) && (n == 1 || (wait(bar_taken, 0) && issue_s(1)));
       for (int i = 0; ok && i < n; ++i) {
         const int st = i & 1;
-        for (int c = 0; ok && c < 4; ++c) {
-          if (!(ok = wait(bar_ds + c, i & 1))) break;
-          mma_sum_quarter<HD>(mine, tDV, tDP, desc_at(g_sum, st * TILE), c, i == 0);
-          mma_sum_quarter<HD>(mine, tDK, tDP + 16, desc_at(q_sum, st * TILE), c, i == 0);
-        }
+        for (int c = 0; ok && c < 4; ++c)
+          if ((ok = wait(bar_p + c, i & 1))) mma_sum_quarter<HD>(mine, tDV, tDP, desc_at(g_sum, st * TILE), c, i == 0);
+        for (int c = 0; ok && c < 4; ++c)
+          if ((ok = wait(bar_ds + c, i & 1)))
+            mma_sum_quarter<HD>(mine, tDK, tDP + 16, desc_at(q_sum, (i % 3) * TILE), c, i == 0);
         if (!ok) break;
         tc_commit_warp(mine, bar_done + st);
         // dP(i+1) overwrites P(i) and dS(i), S(i+2) S(i+1)
@@ -359,7 +365,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int lo = min(max(first - t0, 0), p.TPT) * p.G, hi = min(max(last - t0, 0), p.TPT) * p.G;
         mask = win_low_bits(hi - c0) & ~win_low_bits(lo - c0);
       }
-      if (!(ok = mbar_wait_warp(bar_q + st, (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+      if (!(ok = mbar_wait_warp(bar_g + st, (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       if (!(ok = mbar_wait_warp(bar_s, i & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
       uint32_t r[32];
@@ -375,6 +381,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (full) load_dp<false>(tdp, mask, dp);
       else load_dp<true>(tdp, mask, dp);
       store_cols(tdp, pr);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(bar_p + wg);
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const float4 d = ndelta[c];
@@ -675,7 +684,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 template <int HD>
 cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   constexpr size_t TILE = (HD / 64) * kBox;
-  constexpr size_t smem_kv = 6 * TILE + 2048 + 256 + 1024, smem_q = 7 * TILE + 256 + 1024;
+  constexpr size_t smem_kv = 7 * TILE + 2048 + 256 + 768, smem_q = 7 * TILE + 256 + 1024;
   static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
   cudaError_t e = allow_smem(window_dkv_kernel<HD>, smem_kv, allowed_kv);
   if (e == cudaSuccess) e = allow_smem(window_dq_kernel<HD>, smem_q, allowed_q);
