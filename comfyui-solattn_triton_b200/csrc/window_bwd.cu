@@ -181,7 +181,6 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                   const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                   const __grid_constant__ WinParams p) {
-  pdl_begin();
   constexpr int NBOX = HD / 64;
   constexpr uint32_t TILE = NBOX * kBox;
 
@@ -190,6 +189,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // more is refused)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   if (smem - smem_raw > 768) {
+    pdl_begin();
     if (threadIdx.x == 0) atomicOr(p.err, kErrWaitLoad);
     return;
   }
@@ -212,21 +212,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // key tiles are the slow index: under a causal mask, and with sinks, the first ones
-  // are seen by the most queries, and the longest CTAs start first
-  int id = blockIdx.x;
-  const int hk = id % p.Hk;
-  id /= p.Hk;
-  const int b = id % p.B, kt = id / p.B;
-  const WinSeq seq(p, b);
-  const int j0 = kt * kTile, j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
-  // tokens that see any of them
-  const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
-  const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
-  const int q_begin = ta / p.TPT;
-  const int n = __shfl_sync(0xffffffffu, (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - q_begin : 0, 0);
-
-  if (threadIdx.x == 0) {
+  // the set-up that touches no global memory runs while the grid before this one finishes
+  if (warp == kSoftmax / 32 && lane == 0) {
     mbar_init(bar_kv, 1);
     for (int i = 0; i < 3; ++i) mbar_init(bar_q + i, 1);
     for (int i = 0; i < 2; ++i) {
@@ -242,15 +229,61 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     mbar_init(bar_dp, 1);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
+  }
+  if (warp == kSoftmax / 32 + 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_begin();
+  // key tiles are the slow index: under a causal mask, and with sinks, the first ones
+  // are seen by the most queries, and the longest CTAs start first
+  int id = blockIdx.x;
+  const int hk = id % p.Hk;
+  id /= p.Hk;
+  const int b = id % p.B, kt = id / p.B;
+  const WinSeq seq(p, b);
+  const int j0 = kt * kTile, j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
+  // tokens that see any of them
+  const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
+  const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
+  const int q_begin = ta / p.TPT;
+  const int n = __shfl_sync(0xffffffffu, (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - q_begin : 0, 0);
+
+  auto load_q = [&](int i) {
+    mbar_arrive_expect_tx(bar_q + i % 3, NBOX * p.RT * 128);
+    for (int x = 0; x < NBOX; ++x)
+      tma_load_4d(sQ + (i % 3) * TILE + x * kBox, &tm_q, bar_q + i % 3, x * 64, hk * p.G, (q_begin + i) * p.TPT, b);
+  };
+  auto load_g = [&](int i) {
+    const int st = i & 1, qt = q_begin + i;
+    mbar_arrive_expect_tx(bar_g + st, NBOX * p.RT * 128 + 1024);
+    const int64_t r = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile;
+    bulk_load(sRow + st * 256, p.rows_lse + r, 512, bar_g + st);
+    bulk_load(sRow + st * 256 + 128, p.rows_delta + r, 512, bar_g + st);
+    for (int x = 0; x < NBOX; ++x)
+      tma_load_4d(sG + st * TILE + x * kBox, &tm_do, bar_g + st, x * 64, hk * p.G, qt * p.TPT, b);
+  };
+  // the first loads do not wait for the other warps
+  if (warp == kSoftmax / 32 && lane == 0 && n > 0) {
+    mbar_arrive_expect_tx(bar_kv, 2 * TILE);
+    for (int i = 0; i < NBOX; ++i) tma_load_4d(sK + i * kBox, &tm_k, bar_kv, i * 64, hk, j0, b);
+    load_q(0);
+    for (int i = 0; i < NBOX; ++i) tma_load_4d(sV + i * kBox, &tm_v, bar_kv, i * 64, hk, j0, b);
+    load_g(0);
+    if (n > 1) {
+      load_q(1);
+      load_g(1);
+    }
+    if (n > 2) load_q(2);
   }
   // rows that no box fills are summed over (with P = dS = 0): they have to be finite
   if (p.RT < kTile && n > 0)
     for (int i = 0; i < 5; ++i) zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, kThreads);
   fence_proxy_async_smem();
-  if (warp == kSoftmax / 32 + 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -258,33 +291,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t tS = tmem, tDP = tmem + 128, tDV = tmem + 256, tDK = tmem + 384;
 
   if (warp == kSoftmax / 32) {
-    // ------------------------------------------------------------ TMA producer
+    // ------------------------------------------- TMA producer (after the first loads above)
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(bar_kv, 2 * TILE);
-      for (int i = 0; i < NBOX; ++i) tma_load_4d(sK + i * kBox, &tm_k, bar_kv, i * 64, hk, j0, b);
-      auto load_q = [&](int i) {
-        mbar_arrive_expect_tx(bar_q + i % 3, NBOX * p.RT * 128);
-        for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sQ + (i % 3) * TILE + x * kBox, &tm_q, bar_q + i % 3, x * 64, hk * p.G, (q_begin + i) * p.TPT, b);
-      };
-      auto load_g = [&](int i) {
-        const int st = i & 1, qt = q_begin + i;
-        mbar_arrive_expect_tx(bar_g + st, NBOX * p.RT * 128 + 1024);
-        const int64_t r = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile;
-        bulk_load(sRow + st * 256, p.rows_lse + r, 512, bar_g + st);
-        bulk_load(sRow + st * 256 + 128, p.rows_delta + r, 512, bar_g + st);
-        for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sG + st * TILE + x * kBox, &tm_do, bar_g + st, x * 64, hk * p.G, qt * p.TPT, b);
-      };
-      load_q(0);
-      for (int i = 0; i < NBOX; ++i) tma_load_4d(sV + i * kBox, &tm_v, bar_kv, i * 64, hk, j0, b);
-      load_g(0);
-      int last_q = 0, last_g = 0;
-      if (n > 1) {
-        load_q(last_q = 1);
-        load_g(last_g = 1);
-      }
-      if (n > 2) load_q(last_q = 2);
+      int last_q = min(3, n) - 1, last_g = min(2, n) - 1;
       bool ok = true;
       for (int i = 0; i + 2 < n; ++i) {
         if (!(ok = mbar_wait(bar_done + (i & 1), (i >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
@@ -427,7 +436,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                  const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ WinParams p) {
-  pdl_begin();
   constexpr int NBOX = HD / 64;
   constexpr uint32_t TILE = NBOX * kBox;
 
@@ -451,6 +459,32 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // the set-up that touches no global memory runs while the grid before this one finishes
+  if (warp == kSoftmax / 32 && lane == 0) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(bar_k + i, 1);
+      mbar_init(bar_dq + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_v + i, 1);
+      mbar_init(bar_dp + i, 1);
+      mbar_init(bar_s + i, 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
+    mbar_init(bar_taken, kSoftmax);
+    mbar_init(bar_drain, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
+  }
+  if (warp == kSoftmax / 32 + 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_begin();
   int id = blockIdx.x;
   const int qt = p.nqt - 1 - id % p.nqt;
   id /= p.nqt;
@@ -467,31 +501,36 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int n = __shfl_sync(0xffffffffu, npre + steps.n, 0);
   auto key0 = [&](int i) { return steps.key0(i < npre ? i : i - npre); };
 
-  if (threadIdx.x == 0) {
-    mbar_init(bar_q, 1);
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(bar_k + i, 1);
-      mbar_init(bar_dq + i, 1);
+  auto load_k = [&](int i) {
+    uint64_t* bar = bar_k + i % 3;
+    mbar_arrive_expect_tx(bar, TILE);
+    for (int x = 0; x < NBOX; ++x)
+      tma_load_4d(sK + (i % 3) * TILE + x * kBox, &tm_k, bar, x * 64, hk, key0(i), b);
+  };
+  auto load_v = [&](int i) {
+    uint64_t* bar = bar_v + (i & 1);
+    mbar_arrive_expect_tx(bar, TILE);
+    for (int x = 0; x < NBOX; ++x)
+      tma_load_4d(sV + (i & 1) * TILE + x * kBox, &tm_v, bar, x * 64, hk, key0(i), b);
+  };
+  // the first loads do not wait for the other warps
+  if (warp == kSoftmax / 32 && lane == 0 && n > 0) {
+    mbar_arrive_expect_tx(bar_q, 2 * NBOX * p.RT * 128);
+    for (int x = 0; x < NBOX; ++x) tma_load_4d(sQ + x * kBox, &tm_q, bar_q, x * 64, hk * p.G, t0, b);
+    load_k(0);
+    for (int x = 0; x < NBOX; ++x) tma_load_4d(sG + x * kBox, &tm_do, bar_q, x * 64, hk * p.G, t0, b);
+    load_v(0);
+    if (n > 1) {
+      load_k(1);
+      load_v(1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_v + i, 1);
-      mbar_init(bar_dp + i, 1);
-      mbar_init(bar_s + i, 1);
-    }
-    for (int i = 0; i < 8; ++i) mbar_init(bar_ds + i, kSoftmax / 4);
-    mbar_init(bar_taken, kSoftmax);
-    mbar_init(bar_drain, 1);
-    fence_barrier_init();
+    if (n > 2) load_k(2);
   }
   if (p.RT < kTile && n > 0) {
     zero_rows<HD>(sQ, p.RT, threadIdx.x, kThreads);
     zero_rows<HD>(sG, p.RT, threadIdx.x, kThreads);
   }
   fence_proxy_async_smem();
-  if (warp == kSoftmax / 32 + 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -499,31 +538,9 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t tS = tmem, tDP = tmem + 256, tDQ = tmem + 384;   // two slots of S (dS written over them)
 
   if (warp == kSoftmax / 32) {
-    // ------------------------------------------------------------ TMA producer
+    // ------------------------------------------- TMA producer (after the first loads above)
     if (lane == 0 && n > 0) {
-      auto load_k = [&](int i) {
-        uint64_t* bar = bar_k + i % 3;
-        mbar_arrive_expect_tx(bar, TILE);
-        for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sK + (i % 3) * TILE + x * kBox, &tm_k, bar, x * 64, hk, key0(i), b);
-      };
-      auto load_v = [&](int i) {
-        uint64_t* bar = bar_v + (i & 1);
-        mbar_arrive_expect_tx(bar, TILE);
-        for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(sV + (i & 1) * TILE + x * kBox, &tm_v, bar, x * 64, hk, key0(i), b);
-      };
-      mbar_arrive_expect_tx(bar_q, 2 * NBOX * p.RT * 128);
-      for (int x = 0; x < NBOX; ++x) tma_load_4d(sQ + x * kBox, &tm_q, bar_q, x * 64, hk * p.G, t0, b);
-      load_k(0);
-      for (int x = 0; x < NBOX; ++x) tma_load_4d(sG + x * kBox, &tm_do, bar_q, x * 64, hk * p.G, t0, b);
-      load_v(0);
-      int last_k = 0, last_v = 0;
-      if (n > 1) {
-        load_k(last_k = 1);
-        load_v(last_v = 1);
-      }
-      if (n > 2) load_k(last_k = 2);
+      int last_k = min(3, n) - 1, last_v = min(2, n) - 1;
       bool ok = true;
       for (int i = 0; i + 2 < n; ++i) {
         if (!(ok = mbar_wait(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;

@@ -32,7 +32,6 @@ __global__ void __launch_bounds__(192, 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                   const __grid_constant__ WinParams p) {
-  pdl_begin();
   constexpr int NBOX = HD / 64;            // 64-column (128-byte) boxes per row
   constexpr uint32_t QBOX = 128 * 128;     // a 128-row box
   constexpr uint32_t HBOX = kStep * 128;   // a 64-row box
@@ -56,6 +55,26 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // the set-up that touches no global memory runs while the grid before this one finishes
+  // (bar_pfull counts the threads of the warps with rows: after the tile is known)
+  if (warp == 4 && lane == 0) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_kfull + i, 1);
+      mbar_init(bar_vfull + i, 1);
+      mbar_init(bar_sfull + i, 1);
+      mbar_init(bar_pvdone + i, 1);
+    }
+    mbar_init(bar_drain, 1);
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  pdl_begin();
   // CTA -> (batch, key head, tile, part): a head's tiles together (they share K and V in
   // L2), the last tiles first (under a causal mask they see the most keys)
   int id = blockIdx.x;
@@ -73,19 +92,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int rows = ntok * p.G;                     // rows of this tile that exist
   const int active = (rows + 31) / 32;             // softmax warps that hold any
 
-  if (threadIdx.x == 0) {
-    // the call's error word: nothing else writes it until a wait of some CTA runs out
-    if (blockIdx.x == 0) *p.err = 0;
-    mbar_init(bar_q, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_kfull + i, 1);
-      mbar_init(bar_vfull + i, 1);
-      mbar_init(bar_sfull + i, 1);
-      mbar_init(bar_pfull + i, 32 * active);
-      mbar_init(bar_pvdone + i, 1);
-    }
-    mbar_init(bar_drain, 1);
+  // the call's error word: nothing else writes it until a wait of some CTA runs out
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;
+  // loads in the order of their use: K0 V0 K1 V1 | K(s+2) after QK(s), V(s+2) after PV(s)
+  auto load = [&](int s, bool is_v) {
+    uint64_t* bar = (is_v ? bar_vfull : bar_kfull) + (s & 1);
+    uint8_t* dst = (is_v ? sV : sK) + (s & 1) * SLOT;
+    mbar_arrive_expect_tx(bar, SLOT);
+    for (int i = 0; i < NBOX; ++i)
+      tma_load_4d(dst + i * HBOX, is_v ? &tm_v : &tm_k, bar, i * 64, hk, steps.key0(s_begin + s), b);
+  };
+  if (warp == 4 && lane == 0) {
+    for (int i = 0; i < 2; ++i) mbar_init(bar_pfull + i, 32 * active);
     fence_barrier_init();
+    // the first loads do not wait for the other warps
+    if (nsteps > 0) {
+      mbar_arrive_expect_tx(bar_q, NBOX * p.RT * 128);
+      for (int i = 0; i < NBOX; ++i) tma_load_4d(sQ + i * QBOX, &tm_q, bar_q, i * 64, hk * p.G, t0, b);
+      for (int s = 0; s < min(2, nsteps); ++s) {
+        load(s, false);
+        load(s, true);
+      }
+    }
   }
   // rows of the tile that no box fills (G does not divide 128): finite scores for them
   for (int i = threadIdx.x; i < NBOX * (128 - p.RT) * 8; i += blockDim.x) {
@@ -93,10 +121,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     *reinterpret_cast<uint4*>(sQ + box * QBOX + p.RT * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, 256);
-    tmem_relinquish();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -105,30 +129,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t tO = tmem + 128;    // output accumulator (HD columns)
 
   if (warp == 4) {
-    // ------------------------------------------------------------ TMA producer
-    //   K0 K1 | V0 K2 | V1 K3 | ...  K(s+2) waits for QK(s), V(s) for PV(s-2).
+    // ------------------------------------------- TMA producer (after the first loads above)
     if (lane == 0 && nsteps > 0) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-      mbar_arrive_expect_tx(bar_q, NBOX * p.RT * 128);
-      for (int i = 0; i < NBOX; ++i) tma_load_4d(sQ + i * QBOX, &tm_q, bar_q, i * 64, hk * p.G, t0, b);
-      auto load = [&](int s, bool is_v) {
-        uint64_t* bar = (is_v ? bar_vfull : bar_kfull) + (s & 1);
-        uint8_t* dst = (is_v ? sV : sK) + (s & 1) * SLOT;
-        mbar_arrive_expect_tx(bar, SLOT);
-        for (int i = 0; i < NBOX; ++i)
-          tma_load_4d(dst + i * HBOX, is_v ? &tm_v : &tm_k, bar, i * 64, hk, steps.key0(s_begin + s), b);
-      };
       bool ok = true;
-      int last_k = -1, last_v = -1;
-      for (; last_k + 1 < min(2, nsteps);) load(++last_k, false);
-      for (int s = 0; s < nsteps; ++s) {
-        if (s >= 2 && !(ok = mbar_wait(bar_pvdone + (s & 1), ((s - 2) >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-        load(last_v = s, true);
-        if (s + 2 < nsteps) {
-          if (!(ok = mbar_wait(bar_sfull + (s & 1), (s >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-          load(last_k = s + 2, false);
-        }
+      int last_k = min(2, nsteps) - 1, last_v = last_k;
+      for (int s = 0; s + 2 < nsteps; ++s) {
+        if (!(ok = mbar_wait(bar_sfull + (s & 1), (s >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        load(last_k = s + 2, false);
+        if (!(ok = mbar_wait(bar_pvdone + (s & 1), (s >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        load(last_v = s + 2, true);
       }
       if (!ok) {
         // exit path: every issued copy lands before the CTA's shared memory goes away
