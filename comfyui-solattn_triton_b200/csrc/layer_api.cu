@@ -116,9 +116,28 @@ int window_splits(int64_t tiles, int64_t steps, int64_t row_bytes) {
   return best;
 }
 
+// The gradient's parts, in steps of one CTA (about 2 us each, one CTA per SM): `most` steps of the longest
+// tile, `mean` of all of them, kOpen to open and close a CTA; the joining kernel takes kJoin and moves
+// part_bytes per part there and back (8 MB a step). Measured, forward and gradient (us): 2 heads x 2000
+// causal tokens 84 whole, 65 in parts; 2 x 4000 in a window of 200 with 64 sinks 102 and 69; 8 x 800 53 and 59.
+int gradient_splits(int64_t tiles, int64_t most, double mean, int64_t part_bytes) {
+  constexpr double kOpen = 3, kJoin = 3.5, kSms = 148;
+  int best = 1;
+  double best_cost = 0;
+  for (int n = 1; n <= 16 && (n == 1 || n * 2 <= most); ++n) {
+    const double longest = (double)((most + n - 1) / n) + kOpen, all = (double)tiles * (mean + n * kOpen) / kSms;
+    const double cost = (longest > all ? longest : all) + (n > 1 ? kJoin + n * 2.0 * part_bytes / 8e6 : 0);
+    if (n == 1 || cost < best_cost) {
+      best_cost = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
 struct WinPlan {
   WinParams p;
-  int64_t off_ml, off_o, off_lse, off_delta, fwd_bytes, bwd_bytes;
+  int64_t off_ml, off_o, off_lse, off_delta, off_dq, off_dkv, fwd_bytes, bwd_bytes;
 };
 
 int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, int64_t left,
@@ -157,8 +176,23 @@ int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, in
   w.fwd_bytes = cur;
   const int64_t slots = tiles * kTileRows * (int64_t)sizeof(float);
   w.off_lse = 256;
-  w.off_delta = w.off_lse + slots;
-  w.bwd_bytes = w.off_delta + slots;
+  w.off_delta = w.off_lse + slots;   // (tiles of 128 rows: 512-byte multiples)
+  // gradient: key steps of a query tile, query tiles of a key tile; a causal call without a left bound has
+  // half of them on average, and sinks are seen by every tile
+  const int64_t steps_q = (keys + kTileRows - 1) / kTileRows + 1;
+  const bool bounded = left >= 0 && right >= 0 && left < Tq && right < Tq;
+  const int64_t near = bounded ? (kTileRows + left + right) / p.TPT + 2 : p.nqt;
+  const int64_t tiles_k = near < p.nqt ? near : p.nqt;
+  const double half = left < 0 && right >= 0 ? 0.5 : 1.0;
+  p.split_q = gradient_splits(tiles, steps_q < p.nkt ? steps_q : p.nkt, half * (steps_q < p.nkt ? steps_q : p.nkt),
+                              B * Tq * H * D * 4);
+  p.split_k = gradient_splits(B * Hk * p.nkt, p.sinks > 0 ? p.nqt : tiles_k, half * tiles_k, 2 * B * Tk * Hk * D * 4);
+  cur = up(w.off_delta + slots);
+  w.off_dq = cur;
+  if (p.split_q > 1) cur = up(cur + p.split_q * B * Tq * H * D * (int64_t)sizeof(float));
+  w.off_dkv = cur;
+  if (p.split_k > 1) cur = up(cur + 2 * p.split_k * B * Tk * Hk * D * (int64_t)sizeof(float));
+  w.bwd_bytes = cur;
   return SOLB200_OK;
 }
 
@@ -325,6 +359,11 @@ int32_t solb200_window_attn_backward(const void* dout, const int64_t* dout_strid
   if ((rc = bthd_map(&m.o, dq, D, heads, q_tokens, batch, dqs, p.G, p.TPT, "dq"))) return rc;
   if ((rc = bthd_map(&m.dk, dk, D, kv_heads, kv_tokens, batch, dks, 1, kTileRows, "dk"))) return rc;
   if ((rc = bthd_map(&m.dv, dv, D, kv_heads, kv_tokens, batch, dks, 1, kTileRows, "dv"))) return rc;
+  p.out = static_cast<__nv_bfloat16*>(dq);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  p.part_dq = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_dq);
+  p.part_dkv = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.off_dkv);
   p.lse_in = lse;
   p.o_in = static_cast<const __nv_bfloat16*>(out);
   p.do_in = static_cast<const __nv_bfloat16*>(dout);

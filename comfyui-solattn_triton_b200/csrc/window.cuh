@@ -23,7 +23,7 @@ struct WinParams {
   float scale, s2;          // softmax scale, and times log2(e)
   int* err;
   uint64_t wait_ns;
-  __nv_bfloat16* out;       // split forward: dense [B, Tq, H, D]
+  __nv_bfloat16* out;       // split forward, split dq: dense [B, Tq, H, D]
   float* lse;               // forward: [B, H, Tq] or null
   float* part_o;            // split forward: [nsplit, B, Tq, H, D] unnormalised sums
   float2* part_ml;          // split forward: [nsplit, B, Tq, H] (row maximum in log2 units, row sum)
@@ -34,6 +34,10 @@ struct WinParams {
   float* rows_lse;          // [B, Hk, nqt, 128] lse * log2(e) by tile row (+inf: nothing seen, or no row)
   float* rows_delta;        // [B, Hk, nqt, 128] sum(dO * O) by tile row
   int nkt;                  // key tiles of 128
+  int split_q, split_k;     // parts of a query tile's key steps (dq) and of a key tile's query tiles (dk, dv)
+  float* part_dq;           // [split_q, B, Tq, H, D] if split_q > 1
+  float* part_dkv;          // [split_k, 2 (dv, dk), B, Tk, Hk, D] if split_k > 1
+  __nv_bfloat16 *dk, *dv;   // what the parts are joined into (dq: out)
 };
 
 // A sequence's place: valid keys and the position of query 0.

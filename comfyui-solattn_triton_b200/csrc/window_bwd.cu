@@ -17,6 +17,9 @@
 // for window_dkv_kernel at 4 x 4096 tokens x 24 heads x 128, 1087 keys a row), one TMA warp, one MMA
 // warp, one CTA per SM.
 //
+// Where the tiles are too few to fill the GPU, a tile's walk is divided over split_q (split_k) CTAs,
+// which write their sums in 32 bits; window_grad_join_kernel adds them up in order.
+//
 // window_rows_kernel comes first: -delta and -lse * log2(e) laid out by query tile, -inf for rows
 // that see nothing and for the tile's rows past the last token, which makes their P zero. Its
 // delta carries the rounding of O to bf16, which counts where a row sees few keys (one key: dS
@@ -95,6 +98,49 @@ __device__ __forceinline__ void stage_row(uint32_t taddr, float scale, uint8_t* 
           make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+}
+
+// The same channels in 32 bits straight to a part's row in memory (few tiles: its cost counts little).
+template <int NC>
+__device__ __forceinline__ void store_part(uint32_t taddr, float scale, float* dst, int c0, bool live, bool zero) {
+#pragma unroll 1
+  for (int c = c0; c < c0 + NC; c += 32) {
+    uint32_t r[32];
+    if (!zero) {
+      tmem_ld32(taddr + c, r);
+      tmem_wait_ld();
+    }
+    if (live) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v)
+        *reinterpret_cast<float4*>(dst + c + v * 4) =
+            zero ? make_float4(0.f, 0.f, 0.f, 0.f)
+                 : make_float4(__uint_as_float(r[v * 4]) * scale, __uint_as_float(r[v * 4 + 1]) * scale,
+                               __uint_as_float(r[v * 4 + 2]) * scale, __uint_as_float(r[v * 4 + 3]) * scale);
+    }
+  }
+}
+
+// dq, dk and dv from their parts: blockIdx.y 0 joins dq (split_q parts), 1 dv and 2 dk (split_k parts); 8
+// elements per thread.
+__global__ void __launch_bounds__(256) window_grad_join_kernel(const __grid_constant__ WinParams p, int64_t nq, int64_t nk) {
+  pdl_begin();
+  const int which = blockIdx.y;
+  const int64_t n = which ? nk : nq, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const int parts = which ? p.split_k : p.split_q;
+  if (i >= n || parts == 1) return;
+  const float* src = (which ? p.part_dkv + (which - 1) * nk : p.part_dq) + i;
+  const int64_t step = which ? 2 * nk : nq;
+  float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(src + s * step), y = *reinterpret_cast<const float4*>(src + s * step + 4);
+    a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
+    a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+  }
+  __nv_bfloat16* dst = which == 0 ? p.out : (which == 1 ? p.dv : p.dk);
+  *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
+                                                  pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
 }
 
 // One row per HD / 8 lanes.
@@ -244,14 +290,17 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   int id = blockIdx.x;
   const int hk = id % p.Hk;
   id /= p.Hk;
-  const int b = id % p.B, kt = id / p.B;
+  const int b = id % p.B;
+  id /= p.B;
+  const int split = id % p.split_k, kt = id / p.split_k;
   const WinSeq seq(p, b);
   const int j0 = kt * kTile, j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
   // tokens that see any of them
   const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
   const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
-  const int q_begin = ta / p.TPT;
-  const int n = __shfl_sync(0xffffffffu, (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - q_begin : 0, 0);
+  const int n_all = (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - ta / p.TPT : 0;
+  const int q_begin = ta / p.TPT + (int)((int64_t)n_all * split / p.split_k);
+  const int n = __shfl_sync(0xffffffffu, ta / p.TPT + (int)((int64_t)n_all * (split + 1) / p.split_k) - q_begin, 0);
 
   auto load_q = [&](int i) {
     mbar_arrive_expect_tx(bar_q + i % 3, NBOX * p.RT * 128);
@@ -406,7 +455,12 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
-    if (ok) {
+    if (ok && p.split_k > 1) {
+      constexpr int NC = HD / 2;
+      const int64_t row0 = ((int64_t)split * 2 + (wg < 2 ? 0 : 1)) * p.B * p.Tk;
+      store_part<NC>((wg < 2 ? tDV : tDK) + lane_base, wg < 2 ? 1.f : p.scale,
+                     p.part_dkv + ((row0 + (int64_t)b * p.Tk + j) * p.Hk + hk) * HD, (wg & 1) * NC, j < p.Tk, n == 0);
+    } else if (ok) {
       // two of the four column groups take dV, two dK, half of the channels each; the tiles of V and
       // K are free (every product is complete)
       constexpr int NC = HD / 2;
@@ -414,7 +468,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     n == 0);
       fence_proxy_async_smem();
     }
-    if (named_bar_all(1, kSoftmax, ok) && threadIdx.x == 0) {
+    if (named_bar_all(1, kSoftmax, ok) && p.split_k == 1 && threadIdx.x == 0) {
       for (int i = 0; i < NBOX; ++i) {
         tma_store_4d(&tm_dv, sV + i * kBox, i * 64, hk, j0, b);
         tma_store_4d(&tm_dk, sK + i * kBox, i * 64, hk, j0, b);
@@ -486,6 +540,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   }
   pdl_begin();
   int id = blockIdx.x;
+  const int split = id % p.split_q;
+  id /= p.split_q;
   const int qt = p.nqt - 1 - id % p.nqt;
   id /= p.nqt;
   const int hk = id % p.Hk, b = id / p.Hk;
@@ -496,10 +552,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int rows = ntok * p.G;
   // passes over steps: with 2 .. kFewSteps steps, one pass for delta before the one for dS (a
   // single step has all of a row's P and dP at hand)
-  const bool few = steps.n <= kFewSteps;
-  const int npre = __shfl_sync(0xffffffffu, few && steps.n > 1 ? steps.n : 0, 0);
-  const int n = __shfl_sync(0xffffffffu, npre + steps.n, 0);
-  auto key0 = [&](int i) { return steps.key0(i < npre ? i : i - npre); };
+  const bool few = steps.n <= kFewSteps;   // (not divided: the first part takes all)
+  const int s_begin = few ? 0 : (int)((int64_t)steps.n * split / p.split_q);
+  const int mine_n = few ? (split == 0 ? steps.n : 0) : (int)((int64_t)steps.n * (split + 1) / p.split_q) - s_begin;
+  const int npre = __shfl_sync(0xffffffffu, few && mine_n > 1 ? mine_n : 0, 0);
+  const int n = __shfl_sync(0xffffffffu, npre + mine_n, 0);
+  auto key0 = [&](int i) { return steps.key0(s_begin + (i < npre ? i : i - npre)); };
 
   auto load_k = [&](int i) {
     uint64_t* bar = bar_k + i % 3;
@@ -679,12 +737,15 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
-    if (ok && wg < HD / 32) {
+    if (ok && wg < HD / 32 && p.split_q > 1) {
+      const int64_t orow = ((int64_t)split * p.B * p.Tq + (int64_t)b * p.Tq + t0 + tok) * p.H + hk * p.G + head;
+      store_part<32>(tDQ + lane_base, p.scale, p.part_dq + orow * HD, wg * 32, live, n == 0);
+    } else if (ok && wg < HD / 32) {
       // (the tile of Q is free: every product is complete)
       stage_row<32>(tDQ + lane_base, p.scale, sQ, row, wg * 32, n == 0);
       fence_proxy_async_smem();
     }
-    if (named_bar_all(1, kSoftmax, ok) && threadIdx.x == 0) {
+    if (named_bar_all(1, kSoftmax, ok) && p.split_q == 1 && threadIdx.x == 0) {
       for (int i = 0; i < NBOX; ++i) tma_store_4d(&tm_dq, sQ + i * kBox, i * 64, hk * p.G, t0, b);
       bulk_commit_group();
       bulk_wait_group_read0();
@@ -710,11 +771,17 @@ cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   e = launch_pdl(window_rows_kernel<HD>, dim3((unsigned)(slots * (HD / 8) / 256)), dim3(256), 0, st, p);
   if (e != cudaSuccess) return e;
   // window_dq_kernel leaves refined deltas for window_dkv_kernel
-  e = launch_pdl(window_dq_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nqt)), dim3(kThreads), smem_q, st, m.q,
-                 m.k, m.v, m.dout, m.o, p);
+  const int64_t heads = (int64_t)p.B * p.Hk;
+  e = launch_pdl(window_dq_kernel<HD>, dim3((unsigned)(heads * p.nqt * p.split_q)), dim3(kThreads), smem_q, st, m.q, m.k,
+                 m.v, m.dout, m.o, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(window_dkv_kernel<HD>, dim3((unsigned)((int64_t)p.B * p.Hk * p.nkt)), dim3(kThreads), smem_kv, st,
-                    m.q, m.k, m.v, m.dout, m.dk, m.dv, p);
+  e = launch_pdl(window_dkv_kernel<HD>, dim3((unsigned)(heads * p.nkt * p.split_k)), dim3(kThreads), smem_kv, st, m.q,
+                 m.k, m.v, m.dout, m.dk, m.dv, p);
+  if (e != cudaSuccess || (p.split_q == 1 && p.split_k == 1)) return e;
+  const int64_t nq = p.split_q > 1 ? (int64_t)p.B * p.Tq * p.H * HD : 0;
+  const int64_t nk = p.split_k > 1 ? (int64_t)p.B * p.Tk * p.Hk * HD : 0;
+  const int64_t most = nq > nk ? nq : nk;
+  return launch_pdl(window_grad_join_kernel, dim3((unsigned)((most + 2047) / 2048), 3), dim3(256), 0, st, p, nq, nk);
 }
 
 }  // namespace

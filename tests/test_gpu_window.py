@@ -153,7 +153,16 @@ def test_forward(cuda_device, B, Tq, Tk, H, Hk, D, how):
     _check_forward(*_inputs(B, Tq, Tk, H, Hk, D, seed=Tq + Tk), how)
 
 
-@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,how", [c for c in FORWARD if c[1] <= 333])
+# few tiles with long walks: divided over the query tiles and the key steps
+LONG_GRADIENT = [
+    (1, 1500, 1500, 2, 2, 64, {}),
+    (1, 1100, 1100, 3, 1, 128, dict(left=None, right=None)),
+    (2, 1300, 1300, 2, 1, 64, dict(left=100, sinks=7, lengths=[1300, 700], offsets=[0, 0])),
+    (1, 300, 2500, 2, 2, 128, dict(left=2000, lengths=[2400])),
+]
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,how", [c for c in FORWARD if c[1] <= 333] + LONG_GRADIENT)
 def test_gradient(cuda_device, B, Tq, Tk, H, Hk, D, how):
     q, k, v = _inputs(B, Tq, Tk, H, Hk, D, seed=Tq + 3 * Tk)
     dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(1)).bfloat16()

@@ -44,6 +44,10 @@ def test_window_plan_splits_only_where_tiles_are_few():
     assert rc == 0 and huge == token                     # bounds past every position
     rc, grad = _window_bytes(2, 100, 100, 6, 2, 64, -1, 0, 0, backward=1)
     assert rc == 0 and grad == 256 + 2 * 2 * 2 * 3 * 128 * 4   # two numbers per row of 3 tiles
+    rc, grad = _window_bytes(1, 1500, 1500, 2, 2, 64, -1, 0, 0, backward=1)
+    assert rc == 0 and grad > 256 + 2 * 2 * 12 * 128 * 4 + 2 * 1500 * 2 * 64 * 4   # and parts of the gradients
+    rc, grad = _window_bytes(4, 4096, 4096, 24, 24, 128, 1023, 0, 64, backward=1)
+    assert rc == 0 and grad == 256 + 2 * 4 * 24 * 32 * 128 * 4
 
 
 @pytest.mark.parametrize("args", [(0, 4, 2, 2, 64), (1, 0, 2, 2, 64), (1, 4, 0, 2, 64), (1, 4, 2, 0, 64),
