@@ -50,6 +50,15 @@ struct WinSeq {
   }
 };
 
+// Quotient and remainder of non-negative numbers (unsigned division is the cheaper one); by 1 without any.
+__device__ __forceinline__ int udiv(int a, int b) { return b == 1 ? a : (int)((unsigned)a / (unsigned)b); }
+struct DivMod {
+  int quot, rem;
+  __device__ __forceinline__ DivMod(int a, int b) : quot(udiv(a, b)), rem(a - quot * b) {}
+};
+// First of n steps that part `i` of `parts` takes (n and i * n below 2^31).
+__device__ __forceinline__ int part_begin(int n, int i, int parts) { return parts == 1 ? (i ? n : 0) : udiv(n * i, parts); }
+
 __device__ __forceinline__ int clamp_to(int64_t x, int lo, int hi) {
   return (int)(x < lo ? lo : (x > hi ? hi : x));
 }
@@ -97,6 +106,7 @@ __device__ __forceinline__ uint32_t win_bits(int k0, int lo, int hi, int sinks) 
 // and 0 * NaN would reach the tile's sums: their rows are zeroed in shared memory.
 struct WinUnseen {
   int a0, a1, b0;
+  __device__ explicit WinUnseen(int) : a0(0), a1(0), b0(1 << 30) {}   // none
   __device__ WinUnseen(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
     const int hi = win_hi(p, L, pb);
     a0 = max(0, min(n, p.sinks - k0));

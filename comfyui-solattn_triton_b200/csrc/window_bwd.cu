@@ -287,20 +287,16 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   pdl_begin();
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
   // are seen by the most queries, and the longest CTAs start first
-  int id = blockIdx.x;
-  const int hk = id % p.Hk;
-  id /= p.Hk;
-  const int b = id % p.B;
-  id /= p.B;
-  const int split = id % p.split_k, kt = id / p.split_k;
+  const DivMod by_hk(blockIdx.x, p.Hk), by_b(by_hk.quot, p.B), by_split(by_b.quot, p.split_k);
+  const int hk = by_hk.rem, b = by_b.rem, split = by_split.rem, kt = by_split.quot;
   const WinSeq seq(p, b);
   const int j0 = kt * kTile, j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
   // tokens that see any of them
   const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
   const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
-  const int n_all = (j1 > j0 && tb > ta) ? (tb + p.TPT - 1) / p.TPT - ta / p.TPT : 0;
-  const int q_begin = ta / p.TPT + (int)((int64_t)n_all * split / p.split_k);
-  const int n = __shfl_sync(0xffffffffu, ta / p.TPT + (int)((int64_t)n_all * (split + 1) / p.split_k) - q_begin, 0);
+  const int q_first = udiv(ta, p.TPT), n_all = (j1 > j0 && tb > ta) ? udiv(tb + p.TPT - 1, p.TPT) - q_first : 0;
+  const int q_begin = q_first + part_begin(n_all, split, p.split_k);
+  const int n = __shfl_sync(0xffffffffu, q_first + part_begin(n_all, split + 1, p.split_k) - q_begin, 0);
 
   auto load_q = [&](int i) {
     mbar_arrive_expect_tx(bar_q + i % 3, NBOX * p.RT * 128);
@@ -332,7 +328,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // rows that no box fills are summed over (with P = dS = 0): they have to be finite
   if (p.RT < kTile && n > 0)
     for (int i = 0; i < 5; ++i) zero_rows<HD>(sQ + i * TILE, p.RT, threadIdx.x, kThreads);
-  fence_proxy_async_smem();
+  if (p.RT < kTile) fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -539,12 +535,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tmem_relinquish();
   }
   pdl_begin();
-  int id = blockIdx.x;
-  const int split = id % p.split_q;
-  id /= p.split_q;
-  const int qt = p.nqt - 1 - id % p.nqt;
-  id /= p.nqt;
-  const int hk = id % p.Hk, b = id / p.Hk;
+  const DivMod by_split(blockIdx.x, p.split_q), by_tile(by_split.quot, p.nqt), by_hk(by_tile.quot, p.Hk);
+  const int split = by_split.rem, qt = p.nqt - 1 - by_tile.rem, hk = by_hk.rem, b = by_hk.quot;
   const WinSeq seq(p, b);
   const int t0 = qt * p.TPT, ntok = min(p.TPT, p.Tq - t0);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
@@ -553,8 +545,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   // passes over steps: with 2 .. kFewSteps steps, one pass for delta before the one for dS (a
   // single step has all of a row's P and dP at hand)
   const bool few = steps.n <= kFewSteps;   // (not divided: the first part takes all)
-  const int s_begin = few ? 0 : (int)((int64_t)steps.n * split / p.split_q);
-  const int mine_n = few ? (split == 0 ? steps.n : 0) : (int)((int64_t)steps.n * (split + 1) / p.split_q) - s_begin;
+  const int s_begin = few ? 0 : part_begin(steps.n, split, p.split_q);
+  const int mine_n = few ? (split == 0 ? steps.n : 0) : part_begin(steps.n, split + 1, p.split_q) - s_begin;
   const int npre = __shfl_sync(0xffffffffu, few && mine_n > 1 ? mine_n : 0, 0);
   const int n = __shfl_sync(0xffffffffu, npre + mine_n, 0);
   auto key0 = [&](int i) { return steps.key0(s_begin + (i < npre ? i : i - npre)); };
@@ -588,7 +580,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     zero_rows<HD>(sQ, p.RT, threadIdx.x, kThreads);
     zero_rows<HD>(sG, p.RT, threadIdx.x, kThreads);
   }
-  fence_proxy_async_smem();
+  if (p.RT < kTile) fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -686,7 +678,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t ts = tS + (i & 1) * 128 + lane_base + c0, tdp = tDP + lane_base + c0;
       const bool full = k0 + kTile <= full_hi && (k0 >= full_lo || k0 + kTile <= p.sinks);
       const uint32_t mask = !full && live ? win_bits(k0 + c0, lo, hi, p.sinks) : 0u;
-      ok = mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
+      ok = ok && mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
       tc_fence_after();
       float2 pr[16], dp[16];
       if (ok) {
@@ -708,8 +700,9 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (ok && (i < npre || n == 1))
 #pragma unroll
           for (int c = 0; c < 16; ++c) sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
-        // (every softmax thread comes here at these steps: a failed wait leaves the loop only below)
+        // every softmax thread comes here once: a failed wait leaves the loop only after it
         if (n == 1 || i + 1 == npre) refine();
+        if (!ok && i + 1 < npre) continue;
       }
       if (!ok) break;
       if (i >= npre) {
@@ -717,8 +710,9 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 16; ++c) dp[c] = mul2(pr[c], add2(dp[c], nd));
         store_cols(ts, dp);
-        const WinUnseen unseen(p, seq.L, pa, pb, k0, kTile);
-        if (!full && unseen.any(kTile)) {
+        WinUnseen unseen(0);
+        if (!full) unseen = WinUnseen(p, seq.L, pa, pb, k0, kTile);
+        if (unseen.any(kTile)) {
           // (S(i) is complete, and bar_k was waited for before it was issued)
           if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
           // each column group zeroes the rows of its own quarter of the sum: bar_ds is per group

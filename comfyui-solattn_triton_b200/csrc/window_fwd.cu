@@ -77,18 +77,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   pdl_begin();
   // CTA -> (batch, key head, tile, part): a head's tiles together (they share K and V in
   // L2), the last tiles first (under a causal mask they see the most keys)
-  int id = blockIdx.x;
-  const int split = id % p.nsplit;
-  id /= p.nsplit;
-  const int qt = p.nqt - 1 - id % p.nqt;
-  id /= p.nqt;
-  const int hk = id % p.Hk, b = id / p.Hk;
+  const DivMod by_split(blockIdx.x, p.nsplit), by_tile(by_split.quot, p.nqt), by_hk(by_tile.quot, p.Hk);
+  const int split = by_split.rem, qt = p.nqt - 1 - by_tile.rem, hk = by_hk.rem, b = by_hk.quot;
   const WinSeq seq(p, b);
   const int t0 = qt * p.TPT, ntok = min(p.TPT, p.Tq - t0);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kStep> steps(p, seq.L, pa, pb);
-  const int s_begin = (int)((int64_t)steps.n * split / p.nsplit);
-  const int nsteps = __shfl_sync(0xffffffffu, (int)((int64_t)steps.n * (split + 1) / p.nsplit) - s_begin, 0);
+  const int s_begin = part_begin(steps.n, split, p.nsplit);
+  const int nsteps = __shfl_sync(0xffffffffu, part_begin(steps.n, split + 1, p.nsplit) - s_begin, 0);
   const int rows = ntok * p.G;                     // rows of this tile that exist
   const int active = (rows + 31) / 32;             // softmax warps that hold any
 
@@ -120,7 +116,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int box = i / ((128 - p.RT) * 8), rest = i % ((128 - p.RT) * 8);
     *reinterpret_cast<uint4*>(sQ + box * QBOX + p.RT * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
   }
-  fence_proxy_async_smem();
+  if (p.RT < 128) fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
