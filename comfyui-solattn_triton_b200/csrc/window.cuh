@@ -106,7 +106,6 @@ __device__ __forceinline__ uint32_t win_bits(int k0, int lo, int hi, int sinks) 
 // and 0 * NaN would reach the tile's sums: their rows are zeroed in shared memory.
 struct WinUnseen {
   int a0, a1, b0;
-  __device__ explicit WinUnseen(int) : a0(0), a1(0), b0(1 << 30) {}   // none
   __device__ WinUnseen(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
     const int hi = win_hi(p, L, pb);
     a0 = max(0, min(n, p.sinks - k0));

@@ -148,16 +148,14 @@ template <int HD>
 __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WinParams p) {
   pdl_begin();
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;   // the call's error word
-  constexpr int GL = HD / 8;
+  constexpr int GL = HD / 8, PER_TILE = kTile * GL / 256;   // CTAs per query tile
   const int lg = threadIdx.x % GL;
-  const int64_t slot = ((int64_t)blockIdx.x * 256 + threadIdx.x) / GL;   // [B, Hk, nqt, 128]
-  const int row = (int)(slot & 127);
-  const int64_t tile = slot >> 7;
-  const int qt = (int)(tile % p.nqt);
-  const int64_t bh = tile / p.nqt;
-  const int hk = (int)(bh % p.Hk), b = (int)(bh / p.Hk);
-  const int tok = qt * p.TPT + row / p.G, h = hk * p.G + row % p.G;
-  const bool live = b < p.B && row < p.RT && tok < p.Tq;
+  const int tile = blockIdx.x / PER_TILE, row = (blockIdx.x % PER_TILE) * (256 / GL) + threadIdx.x / GL;
+  const int64_t slot = (int64_t)tile * kTile + row;         // [B, Hk, nqt, 128]
+  const DivMod by_tile(tile, p.nqt), by_hk(by_tile.quot, p.Hk), by_g(row, p.G);
+  const int hk = by_hk.rem, b = by_hk.quot;
+  const int tok = by_tile.rem * p.TPT + by_g.quot, h = hk * p.G + by_g.rem;
+  const bool live = row < p.RT && tok < p.Tq;
   float d = 0.f, neg = -INFINITY;
   if (live) {
     const uint4 wo = __ldg(reinterpret_cast<const uint4*>(p.o_in + b * p.os[0] + tok * p.os[1] + h * p.os[2]) + lg);
@@ -173,7 +171,7 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   }
 #pragma unroll
   for (int o = GL / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  if (lg == 0 && b < p.B) {
+  if (lg == 0) {
     p.rows_lse[slot] = neg;
     p.rows_delta[slot] = neg == -INFINITY ? 0.f : -d;
   }
@@ -658,9 +656,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const float neg = p.rows_lse[slot];
     float ndelta = p.rows_delta[slot];
     float sum = 0.f;   // of P dP over this thread's columns, for delta
+    bool owes = few && n > 0;
     // delta of the row from its four threads' parts, for this kernel and for window_dkv_kernel; the
     // parts meet in dQ's columns, which the first dQ product overwrites later
     auto refine = [&]() {
+      owes = false;
       tmem_st1(tDQ + lane_base + wg, __float_as_uint(sum));
       tmem_wait_st();
       tc_fence_before();
@@ -678,57 +678,53 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t ts = tS + (i & 1) * 128 + lane_base + c0, tdp = tDP + lane_base + c0;
       const bool full = k0 + kTile <= full_hi && (k0 >= full_lo || k0 + kTile <= p.sinks);
       const uint32_t mask = !full && live ? win_bits(k0 + c0, lo, hi, p.sinks) : 0u;
-      ok = ok && mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
+      if (!(ok = mbar_wait_warp(bar_s + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
       tc_fence_after();
       float2 pr[16], dp[16];
-      if (ok) {
+      {
         uint32_t r[32];
         tmem_ld32(ts, r);
         tmem_wait_ld();
         if (full) probs<false>(r, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
         else probs<true>(r, p.s2, mask, pr, [&](int) { return make_float4(neg, neg, neg, neg); });
-        ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns);
-        tc_fence_after();
       }
-      if (ok) {
-        if (full) load_dp<false>(tdp, mask, dp);
-        else load_dp<true>(tdp, mask, dp);
-        tc_fence_before();
-        mbar_arrive(bar_taken);
-      }
-      if (few) {
-        if (ok && (i < npre || n == 1))
+      if (!(ok = mbar_wait_warp(bar_dp + (i & 1), (i >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+      tc_fence_after();
+      if (full) load_dp<false>(tdp, mask, dp);
+      else load_dp<true>(tdp, mask, dp);
+      tc_fence_before();
+      mbar_arrive(bar_taken);
+      if (few && (i < npre || n == 1)) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
-        // every softmax thread comes here once: a failed wait leaves the loop only after it
+        for (int c = 0; c < 16; ++c) sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
         if (n == 1 || i + 1 == npre) refine();
-        if (!ok && i + 1 < npre) continue;
       }
-      if (!ok) break;
       if (i >= npre) {
         const float2 nd = make_float2(ndelta, ndelta);
 #pragma unroll
         for (int c = 0; c < 16; ++c) dp[c] = mul2(pr[c], add2(dp[c], nd));
         store_cols(ts, dp);
-        WinUnseen unseen(0);
-        if (!full) unseen = WinUnseen(p, seq.L, pa, pb, k0, kTile);
-        if (unseen.any(kTile)) {
-          // (S(i) is complete, and bar_k was waited for before it was issued)
-          if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
-          // each column group zeroes the rows of its own quarter of the sum: bar_ds is per group
-          uint8_t* tile = sK + (i % 3) * TILE;
-          for (int c = threadIdx.x & 127; c < 32 * NBOX * 8; c += 128) {
-            const int r = c0 + c / (NBOX * 8), x = c % (NBOX * 8);
-            if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
-              *reinterpret_cast<uint4*>(tile + (x >> 3) * kBox + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+        if (!full) {
+          const WinUnseen unseen(p, seq.L, pa, pb, k0, kTile);
+          if (unseen.any(kTile)) {
+            // (S(i) is complete, and bar_k was waited for before it was issued)
+            if (!(ok = mbar_wait_warp(bar_k + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+            // each column group zeroes the rows of its own quarter of the sum: bar_ds is per group
+            uint8_t* tile = sK + (i % 3) * TILE;
+            for (int c = threadIdx.x & 127; c < 32 * NBOX * 8; c += 128) {
+              const int r = c0 + c / (NBOX * 8), x = c % (NBOX * 8);
+              if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
+                *reinterpret_cast<uint4*>(tile + (x >> 3) * kBox + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
           }
-          fence_proxy_async_smem();
         }
         tmem_wait_st();
       }
       tc_fence_before();
       mbar_arrive(bar_ds + (i & 1) * 4 + wg);
     }
+    if (owes) named_bar_sync(1, kSoftmax);   // (a wait failed before the refinement: take part in its barrier)
     if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok && wg < HD / 32 && p.split_q > 1) {
