@@ -23,8 +23,9 @@
 // window_rows_kernel comes first: -delta and -lse * log2(e) laid out by query tile, -inf for rows
 // that see nothing and for the tile's rows past the last token, which makes their P zero. Its
 // delta carries the rounding of O to bf16, which counts where a row sees few keys (one key: dS
-// is exactly zero). For tiles of up to kFewSteps steps window_dq_kernel therefore forms delta =
-// sum(P dP) in 32 bits first, and leaves it for window_dkv_kernel.
+// is zero). For tiles of up to kFewSteps steps window_dq_kernel therefore forms delta =
+// sum(P dP) / sum(P) in 32 bits first (sum(P) is 1 up to the rounding of lse), and leaves it for
+// window_dkv_kernel.
 #include "fwd_common.cuh"
 #include "window.cuh"
 
@@ -655,21 +656,27 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int64_t slot = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile + row;
     const float neg = p.rows_lse[slot];
     float ndelta = p.rows_delta[slot];
-    float sum = 0.f;   // of P dP over this thread's columns, for delta
+    float sum = 0.f, psum = 0.f;   // of P dP and P over this thread's columns, for delta
     bool owes = few && n > 0;
     // delta of the row from its four threads' parts, for this kernel and for window_dkv_kernel; the
     // parts meet in dQ's columns, which the first dQ product overwrites later
     auto refine = [&]() {
       owes = false;
       tmem_st1(tDQ + lane_base + wg, __float_as_uint(sum));
+      tmem_st1(tDQ + lane_base + 4 + wg, __float_as_uint(psum));
       tmem_wait_st();
       tc_fence_before();
       named_bar_sync(1, kSoftmax);
       tc_fence_after();
-      uint32_t r[4];
+      uint32_t r[4], q[4];
       tmem_ld4(tDQ + lane_base, r);
+      tmem_ld4(tDQ + lane_base + 4, q);
       tmem_wait_ld();
-      ndelta = -((__uint_as_float(r[0]) + __uint_as_float(r[1])) + (__uint_as_float(r[2]) + __uint_as_float(r[3])));
+      auto total = [](const uint32_t (&x)[4]) {
+        return (__uint_as_float(x[0]) + __uint_as_float(x[1])) + (__uint_as_float(x[2]) + __uint_as_float(x[3]));
+      };
+      const float weights = total(q);
+      ndelta = weights == 0.f ? 0.f : -total(r) / weights;   // (0: the row sees nothing)
       if (wg == 0) p.rows_delta[slot] = ndelta;
     };
     bool ok = true;
@@ -696,7 +703,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_arrive(bar_taken);
       if (few && (i < npre || n == 1)) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
+        for (int c = 0; c < 16; ++c) {
+          sum = fmaf(pr[c].x, dp[c].x, fmaf(pr[c].y, dp[c].y, sum));
+          psum += pr[c].x + pr[c].y;
+        }
         if (n == 1 || i + 1 == npre) refine();
       }
       if (i >= npre) {

@@ -177,6 +177,16 @@ def test_gradient(cuda_device, B, Tq, Tk, H, Hk, D, how):
         _check(a, w, bd, name)
 
 
+def test_one_key_per_row_has_no_score_gradient(cuda_device):
+    """Rows that see a single key: P = 1, dS = 0. dq and dk are what fp32 leaves of dP - delta: a
+    few units of 2^-24 of the dot product dO . V (sqrt(D) here) times K."""
+    q, k, v = (t.cuda() for t in _inputs(2, 70, 70, 2, 2, 64, seed=13))
+    for how in (dict(left=0), dict(lengths=torch.tensor([1, 1], dtype=torch.int32).cuda(), right=None)):
+        out, lse = solb200.window_attn(q, k, v, return_lse=True, **how)
+        dq, dk, dv = solb200.window_attn_backward(torch.randn_like(q), q, k, v, out, lse, **how)
+        assert dq.abs().max() <= 2.0 ** -17 and dk.abs().max() <= 70 * 2.0 ** -17 and dv.any()
+
+
 def test_gradient_against_differences(cuda_device):
     """The definition differenced in 64 bits along random directions: off from the kernels'
     gradient by no more than the gradient's own bounds along that direction (h^2 terms are 1e-8)."""
