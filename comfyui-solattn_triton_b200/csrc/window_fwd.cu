@@ -8,16 +8,20 @@
 //
 // The online softmax keeps a per-row reference maximum that is raised only when a step
 // exceeds it by more than 2^8 (sums stay in 32 bits; P is rounded to bf16 for the tensor
-// cores, a relative 2^-9 per weight). Two slots for K, V and scores:
+// cores, at most a relative 2^-8 per weight). Two slots for K, V and scores:
 //   MMA issuer:  QK(0) QK(1) | PV(0) QK(2) | PV(1) QK(3) | ...
 // Warps 0-3 softmax and epilogue (thread = row = TMEM lane; a warp without rows takes no
 // part), warp 4 TMA, warp 5 TMEM and MMA. 96 KB of shared memory and 256 TMEM columns: two CTAs per SM.
 //
 // When the tiles are too few to fill the GPU (single tokens, short chunks against a long
 // cache), the steps are divided over nsplit CTAs, which write their unnormalised sums, maxima
-// and row sums; join_kernel joins them in order.
+// and row sums; window_join_kernel joins them in order.
 //
 // Keys that no row of the tile sees may hold anything (WinUnseen).
+//
+// Measured on a B200, 40 heads x 128: 32760 queries seeing about 5940 keys each 3.5 ms (1.14 PFLOP/s; 4.07 ms
+// and 0.98 at the power cap), bound by one CTA's softmax and the other's products taking turns
+// (tensor pipe 59 % busy, exponentials 60 %); one token over 262001 keys 755 us (7.1 TB/s).
 #include "fwd_common.cuh"
 #include "window.cuh"
 

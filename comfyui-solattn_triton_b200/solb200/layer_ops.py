@@ -291,6 +291,22 @@ def _device_error(ws, stream, what):
     check(lib().solb200_read_device_error(ws.data_ptr(), ctypes.byref(code), stream), what)
 
 
+# The device error word of calls that need no other workspace, by device and stream: calls of one
+# stream run one after the other, and each clears it first.
+_ERROR_WORDS = {}
+
+
+def _workspace(nbytes, q, index, stream):
+    if nbytes > 256:
+        return torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = _ERROR_WORDS.get((index, stream))
+    if ws is None:
+        ws = torch.empty(256, dtype=torch.uint8, device=q.device)
+        if not torch.cuda.is_current_stream_capturing():     # (a graph's memory is the graph's)
+            _ERROR_WORDS[(index, stream)] = ws
+    return ws
+
+
 def _window_forward(q, k, v, left, right, sinks, scale, lengths, offsets, want_lse):
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
     B, Tq, _, H, _, D = plan.place[:6]
@@ -301,8 +317,8 @@ def _window_forward(q, k, v, left, right, sinks, scale, lengths, offsets, want_l
     with _on(index):
         out = q.new_empty((B, Tq, H, D))
         lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
-        ws = torch.empty(plan.bytes, dtype=torch.uint8, device=q.device)
         stream = _raw_stream(index)
+        ws = _workspace(plan.bytes, q, index, stream)
         rc = lib().solb200_window_attn(
             q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, v.data_ptr(), plan.vs, out.data_ptr(), _ptr(lse),
             _ptr(lengths), _ptr(offsets), *plan.place, ws.data_ptr(), plan.bytes, stream)
