@@ -17,7 +17,7 @@
 // TMA warp, one MMA warp, one CTA per SM.
 //
 // Measured on a B200, 4 x 4096 tokens x 24 heads x 128, about 1000 keys a row: window_dq_kernel 373 us,
-// window_dkv_kernel 489 us, 0.68 and 0.70 PFLOP/s of products executed. An iteration takes 2700 and
+// window_dkv_kernel 489 us, 0.91 PFLOP/s of products executed each. An iteration takes 2700 and
 // 3200 cycles against 1536 and 2048 of products: the softmax threads are busy for 2400 and 2700 of
 // them, and only what the barriers allow runs at the same time.
 //
@@ -291,9 +291,17 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // key tiles are the slow index: under a causal mask, and with sinks, the first ones
   // are seen by the most queries, and the longest CTAs start first
   const DivMod by_hk(blockIdx.x, p.Hk), by_b(by_hk.quot, p.B), by_split(by_b.quot, p.split_k);
-  const int hk = by_hk.rem, b = by_b.rem, split = by_split.rem, kt = by_split.quot;
+  const int hk = by_hk.rem, b = by_b.rem, split = by_split.rem, j0 = by_split.quot * kTile;
+  // the first loads wait neither for the rest of the arithmetic nor for the other warps
+  if (warp == kSoftmax / 32 && lane == 0) {
+    mbar_arrive_expect_tx(bar_kv, 2 * TILE);
+    for (int i = 0; i < NBOX; ++i) {
+      tma_load_4d(sK + i * kBox, &tm_k, bar_kv, i * 64, hk, j0, b);
+      tma_load_4d(sV + i * kBox, &tm_v, bar_kv, i * 64, hk, j0, b);
+    }
+  }
   const WinSeq seq(p, b);
-  const int j0 = kt * kTile, j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
+  const int j1 = min(j0 + kTile, seq.L);   // keys [j0, j1) of this tile count
   // tokens that see any of them
   const int ta = p.right < 0 ? 0 : clamp_to((int64_t)j0 - p.right - seq.off, 0, p.Tq);
   const int tb = (p.left < 0 || j0 < p.sinks) ? p.Tq : clamp_to((int64_t)j1 - 1 + p.left - seq.off + 1, 0, p.Tq);
@@ -315,12 +323,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int x = 0; x < NBOX; ++x)
       tma_load_4d(sG + st * TILE + x * kBox, &tm_do, bar_g + st, x * 64, hk * p.G, qt * p.TPT, b);
   };
-  // the first loads do not wait for the other warps
   if (warp == kSoftmax / 32 && lane == 0 && n > 0) {
-    mbar_arrive_expect_tx(bar_kv, 2 * TILE);
-    for (int i = 0; i < NBOX; ++i) tma_load_4d(sK + i * kBox, &tm_k, bar_kv, i * 64, hk, j0, b);
     load_q(0);
-    for (int i = 0; i < NBOX; ++i) tma_load_4d(sV + i * kBox, &tm_v, bar_kv, i * 64, hk, j0, b);
     load_g(0);
     if (n > 1) {
       load_q(1);
@@ -340,6 +344,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (warp == kSoftmax / 32) {
     // ------------------------------------------- TMA producer (after the first loads above)
+    if (lane == 0 && n == 0) mbar_wait(bar_kv, 0, p.err, kErrWaitDrain);
     if (lane == 0 && n > 0) {
       int last_q = min(3, n) - 1, last_g = min(2, n) - 1;
       bool ok = true;
@@ -452,7 +457,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       tc_fence_before();
       mbar_arrive(bar_ds + wg);
     }
-    if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
+    // (without iterations: the loads of K and V, whose tiles take the zeros, have landed)
+    if (ok) ok = mbar_wait_warp(n > 0 ? bar_drain : bar_kv, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok && p.split_k > 1) {
       constexpr int NC = HD / 2;
@@ -540,8 +546,16 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   pdl_begin();
   const DivMod by_split(blockIdx.x, p.split_q), by_tile(by_split.quot, p.nqt), by_hk(by_tile.quot, p.Hk);
   const int split = by_split.rem, qt = p.nqt - 1 - by_tile.rem, hk = by_hk.rem, b = by_hk.quot;
-  const WinSeq seq(p, b);
   const int t0 = qt * p.TPT, ntok = min(p.TPT, p.Tq - t0);
+  // the first loads wait neither for the rest of the arithmetic nor for the other warps
+  if (warp == kSoftmax / 32 && lane == 0) {
+    mbar_arrive_expect_tx(bar_q, 2 * NBOX * p.RT * 128);
+    for (int x = 0; x < NBOX; ++x) {
+      tma_load_4d(sQ + x * kBox, &tm_q, bar_q, x * 64, hk * p.G, t0, b);
+      tma_load_4d(sG + x * kBox, &tm_do, bar_q, x * 64, hk * p.G, t0, b);
+    }
+  }
+  const WinSeq seq(p, b);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kTile> steps(p, seq.L, pa, pb);
   const int rows = ntok * p.G;
@@ -566,12 +580,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     for (int x = 0; x < NBOX; ++x)
       tma_load_4d(sV + (i & 1) * TILE + x * kBox, &tm_v, bar, x * 64, hk, key0(i), b);
   };
-  // the first loads do not wait for the other warps
   if (warp == kSoftmax / 32 && lane == 0 && n > 0) {
-    mbar_arrive_expect_tx(bar_q, 2 * NBOX * p.RT * 128);
-    for (int x = 0; x < NBOX; ++x) tma_load_4d(sQ + x * kBox, &tm_q, bar_q, x * 64, hk * p.G, t0, b);
     load_k(0);
-    for (int x = 0; x < NBOX; ++x) tma_load_4d(sG + x * kBox, &tm_do, bar_q, x * 64, hk * p.G, t0, b);
     load_v(0);
     if (n > 1) {
       load_k(1);
@@ -592,6 +602,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
   if (warp == kSoftmax / 32) {
     // ------------------------------------------- TMA producer (after the first loads above)
+    if (lane == 0 && n == 0) mbar_wait(bar_q, 0, p.err, kErrWaitDrain);
     if (lane == 0 && n > 0) {
       int last_k = min(3, n) - 1, last_v = min(2, n) - 1;
       bool ok = true;
@@ -739,7 +750,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_arrive(bar_ds + (i & 1) * 4 + wg);
     }
     if (owes) named_bar_sync(1, kSoftmax);   // (a wait failed before the refinement: take part in its barrier)
-    if (ok && n > 0) ok = mbar_wait_warp(bar_drain, 0, p.err, kErrWaitEpilogue, p.wait_ns);
+    // (without iterations: the load of Q, whose tile takes the zeros, has landed)
+    if (ok) ok = mbar_wait_warp(n > 0 ? bar_drain : bar_q, 0, p.err, kErrWaitEpilogue, p.wait_ns);
     tc_fence_after();
     if (ok && wg < HD / 32 && p.split_q > 1) {
       const int64_t orow = ((int64_t)split * p.B * p.Tq + (int64_t)b * p.Tq + t0 + tok) * p.H + hk * p.G + head;

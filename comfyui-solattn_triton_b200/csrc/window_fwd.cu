@@ -70,6 +70,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(bar_pvdone + i, 1);
     }
     mbar_init(bar_drain, 1);
+    fence_barrier_init();
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -83,8 +84,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // L2), the last tiles first (under a causal mask they see the most keys)
   const DivMod by_split(blockIdx.x, p.nsplit), by_tile(by_split.quot, p.nqt), by_hk(by_tile.quot, p.Hk);
   const int split = by_split.rem, qt = p.nqt - 1 - by_tile.rem, hk = by_hk.rem, b = by_hk.quot;
-  const WinSeq seq(p, b);
   const int t0 = qt * p.TPT, ntok = min(p.TPT, p.Tq - t0);
+  // the first loads wait neither for the rest of the arithmetic nor for the other warps
+  if (warp == 4 && lane == 0) {
+    mbar_arrive_expect_tx(bar_q, NBOX * p.RT * 128);
+    for (int i = 0; i < NBOX; ++i) tma_load_4d(sQ + i * QBOX, &tm_q, bar_q, i * 64, hk * p.G, t0, b);
+  }
+  const WinSeq seq(p, b);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kStep> steps(p, seq.L, pa, pb);
   const int s_begin = part_begin(steps.n, split, p.nsplit);
@@ -105,14 +111,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (warp == 4 && lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(bar_pfull + i, 32 * active);
     fence_barrier_init();
-    // the first loads do not wait for the other warps
-    if (nsteps > 0) {
-      mbar_arrive_expect_tx(bar_q, NBOX * p.RT * 128);
-      for (int i = 0; i < NBOX; ++i) tma_load_4d(sQ + i * QBOX, &tm_q, bar_q, i * 64, hk * p.G, t0, b);
-      for (int s = 0; s < min(2, nsteps); ++s) {
-        load(s, false);
-        load(s, true);
-      }
+    for (int s = 0; s < min(2, nsteps); ++s) {
+      load(s, false);
+      load(s, true);
     }
   }
   // rows of the tile that no box fills (G does not divide 128): finite scores for them
@@ -130,6 +131,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (warp == 4) {
     // ------------------------------------------- TMA producer (after the first loads above)
+    if (lane == 0 && nsteps == 0) mbar_wait(bar_q, 0, p.err, kErrWaitDrain);
     if (lane == 0 && nsteps > 0) {
       bool ok = true;
       int last_k = min(2, nsteps) - 1, last_v = last_k;
@@ -238,9 +240,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_before();
         mbar_arrive(bar_pfull + slot);
       }
-      if (ok && nsteps > 0) {
-        ok = mbar_wait_warp(bar_pvdone + ((nsteps - 1) & 1), ((nsteps - 1) >> 1) & 1, p.err, kErrWaitEpilogue,
-                            p.wait_ns);
+      if (ok) {
+        // (without steps: the load of Q, whose tile takes the zeros, has landed)
+        ok = nsteps > 0 ? mbar_wait_warp(bar_pvdone + ((nsteps - 1) & 1), ((nsteps - 1) >> 1) & 1, p.err,
+                                         kErrWaitEpilogue, p.wait_ns)
+                        : mbar_wait_warp(bar_q, 0, p.err, kErrWaitEpilogue, p.wait_ns);
         tc_fence_after();
       }
       const bool none = l_sum == 0.f;              // nothing seen (a NaN row is not that)
