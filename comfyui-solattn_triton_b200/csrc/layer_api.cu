@@ -87,7 +87,7 @@ int32_t rope_params(RopeParams& p, const void* q, const int64_t* qs, const void*
 // ------------------------------------------------------------- windowed attention
 
 constexpr int kSlots = 148 * 2;   // forward CTAs resident on the GPU
-constexpr int kStepKeys = 64, kTileRows = 128, kFewRows = 32;
+constexpr int kStepKeys = 64, kTileRows = 128;
 
 // Parts of the key axis: the count with the least estimated time, in steps of 64 keys of one CTA
 // (about a microsecond, whether the tensor cores or memory set the pace). The CTAs run in waves
@@ -141,7 +141,7 @@ struct WinPlan {
 };
 
 int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, int64_t left,
-                    int64_t right, int64_t sinks, bool backward) {
+                    int64_t right, int64_t sinks) {
   if (B < 1 || Tq < 1 || Tk < 1 || H < 1 || Hk < 1) return invalid("batch, tokens and heads must be >= 1");
   if (D != 64 && D != 128) return invalid("head_dim must be 64 or 128");
   if (B > 65536 || Tq > kMost || Tk > kMost || H > 65536) return invalid("batch, tokens or heads too large");
@@ -151,8 +151,7 @@ int32_t window_plan(WinPlan& w, int64_t B, int64_t Tq, int64_t Tk, int64_t H, in
   p = WinParams{};
   p.B = (int)B; p.Tq = (int)Tq; p.Tk = (int)Tk; p.H = (int)H; p.Hk = (int)Hk;
   p.G = (int)(H / Hk);
-  p.few = !backward && Tq * p.G <= kFewRows;
-  p.TPT = (p.few ? kFewRows : kTileRows) / p.G;
+  p.TPT = kTileRows / p.G;
   p.RT = p.TPT * p.G;
   p.nqt = (int)((Tq + p.TPT - 1) / p.TPT);
   p.nkt = (int)((Tk + kTileRows - 1) / kTileRows);
@@ -299,7 +298,7 @@ int32_t solb200_window_attn_workspace(int64_t batch, int64_t q_tokens, int64_t k
                                       int32_t backward, int64_t* bytes) {
   if (!bytes) return invalid("null pointer");
   WinPlan w;
-  const int32_t rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks, backward != 0);
+  const int32_t rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks);
   if (rc) return rc;
   *bytes = backward ? w.bwd_bytes : w.fwd_bytes;
   return SOLB200_OK;
@@ -314,7 +313,7 @@ int32_t solb200_window_attn(const void* q, const int64_t* q_strides, const void*
   if (rc) return rc;
   WinPlan w;
   WinMaps m;
-  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks, false))) return rc;
+  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks))) return rc;
   if (!out || !aligned16(out)) return set_last_error(SOLB200_ERR_ALIGNMENT, "out: null or not 16-byte aligned");
   if ((rc = window_common(w, m, q, q_strides, k, k_strides, v, v_strides, lengths, offsets, batch, q_tokens,
                           kv_tokens, heads, kv_heads, head_dim, scale, kStepKeys, workspace, workspace_bytes,
@@ -344,7 +343,7 @@ int32_t solb200_window_attn_backward(const void* dout, const int64_t* dout_strid
   if (rc) return rc;
   WinPlan w;
   WinMaps m;
-  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks, true))) return rc;
+  if ((rc = window_plan(w, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim, left, right, sinks))) return rc;
   if ((rc = check_rows16("dout", dout, dout_strides, batch, q_tokens, heads, 2, true))) return rc;
   if ((rc = check_rows16("out", out, out_strides, batch, q_tokens, heads, 2, true))) return rc;
   if (!lse || !dq || !dk || !dv || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))

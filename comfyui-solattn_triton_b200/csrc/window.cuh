@@ -15,7 +15,6 @@ struct WinParams {
   int B, Tq, Tk, H, Hk;
   int G;                    // query heads per key head (H / Hk), 1..128
   int TPT, RT, nqt;         // tokens and rows (TPT * G) of a query tile, tiles per (b, key head)
-  int few;                  // forward: tiles of at most 32 rows (Tq * G <= 32)
   int nsplit;               // forward: parts of the key axis, joined by a second kernel
   int64_t left, right;      // < 0: no bound
   int sinks;

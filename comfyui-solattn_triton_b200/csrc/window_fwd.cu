@@ -8,24 +8,20 @@
 //
 // The online softmax keeps a per-row reference maximum that is raised only when a step
 // exceeds it by more than 2^8 (sums stay in 32 bits; P is rounded to bf16 for the tensor
-// cores, at most a relative 2^-8 per weight). Two slots of scores:
+// cores, at most a relative 2^-8 per weight). Two slots for K, V and scores:
 //   MMA issuer:  QK(0) QK(1) | PV(0) QK(2) | PV(1) QK(3) | ...
 // Warps 0-3 softmax and epilogue (thread = row = TMEM lane; a warp without rows takes no
-// part), warp 4 TMA, warp 5 TMEM and MMA. 96 to 106 KB of shared memory and 256 TMEM columns: two CTAs per SM.
+// part), warp 4 TMA, warp 5 TMEM and MMA. 96 KB of shared memory and 256 TMEM columns: two CTAs per SM.
 //
 // When the tiles are too few to fill the GPU (single tokens, short chunks against a long
 // cache), the steps are divided over nsplit CTAs, which write their unnormalised sums, maxima
-// and row sums; window_join_kernel joins them in order. A call of at most 32 rows per key head (single
-// tokens) waits for its loads above all: its tile of Q keeps 32 rows (the products read on into K's
-// slots, for rows that nobody reads), which leaves room for a third step of K and V in flight (six of
-// head_dim 64). Measured against two (us): 16 ragged caches and a window of 4096 keys 48 -> 44.5, four caches of 16384
-// keys and head_dim 64 37 -> 35; where the loads of all CTAs already fill the memory pipe, 262001 keys, 746 -> 761.
+// and row sums; window_join_kernel joins them in order.
 //
 // Keys that no row of the tile sees may hold anything (WinUnseen).
 //
 // Measured on a B200, 40 heads x 128: 32760 queries seeing about 5940 keys each 3.5 ms (1.14 PFLOP/s; 4.07 ms
 // and 0.98 at the power cap), bound by one CTA's softmax and the other's products taking turns
-// (tensor pipe 59 % busy, exponentials 60 %); one token over 262001 keys 761 us (7.05 TB/s).
+// (tensor pipe 59 % busy, exponentials 60 %); one token over 262001 keys 755 us (7.1 TB/s).
 #include "fwd_common.cuh"
 #include "window.cuh"
 
@@ -35,25 +31,15 @@ namespace {
 
 constexpr int kStep = 64;
 
-// FEW: tiles of at most 32 rows.
-template <int HD, bool FEW>
-struct FwdShape {
-  static constexpr int NBOX = HD / 64;                        // 64-column (128-byte) boxes per row
-  static constexpr int SLOTS = !FEW ? 2 : (HD == 128 ? 3 : 6);   // steps of K and V in flight
-  static constexpr int ROWS = FEW ? 32 : 128;                 // rows of Q in shared memory
-  static constexpr uint32_t QBOX = ROWS * 128, HBOX = kStep * 128;
-  static constexpr uint32_t SLOT = NBOX * HBOX;               // one step of K (or V)
-  static constexpr size_t SMEM = NBOX * QBOX + 2 * SLOTS * SLOT + 512 + 1024;
-};
-
-template <int HD, bool FEW>
+template <int HD>
 __global__ void __launch_bounds__(192, 2)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                   const __grid_constant__ WinParams p) {
-  using Shape = FwdShape<HD, FEW>;
-  constexpr int NBOX = Shape::NBOX, SLOTS = Shape::SLOTS;
-  constexpr uint32_t QBOX = Shape::QBOX, HBOX = Shape::HBOX, SLOT = Shape::SLOT;
+  constexpr int NBOX = HD / 64;            // 64-column (128-byte) boxes per row
+  constexpr uint32_t QBOX = 128 * 128;     // a 128-row box
+  constexpr uint32_t HBOX = kStep * 128;   // a 64-row box
+  constexpr uint32_t SLOT = NBOX * HBOX;   // one step of K (or V)
   constexpr uint32_t IDESC_QK = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 0, 128, 64);
   constexpr uint32_t IDESC_PV = make_idesc(kFmtF32, kFmtBF16, kFmtBF16, 0, 1, 128, HD);
 
@@ -61,18 +47,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + NBOX * QBOX;
-  uint8_t* sV = sK + SLOTS * SLOT;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + SLOTS * SLOT);
+  uint8_t* sV = sK + 2 * SLOT;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * SLOT);
   uint64_t* bar_q = bars + 0;
-  uint64_t* bar_sfull = bars + 1;          // [2] by slot of scores
-  uint64_t* bar_pfull = bars + 3;
-  uint64_t* bar_pvdone = bars + 5;
-  uint64_t* bar_drain = bars + 7;
-  uint64_t* bar_kfull = bars + 8;          // [SLOTS] each
-  uint64_t* bar_kfree = bars + 8 + SLOTS;
-  uint64_t* bar_vfull = bars + 8 + 2 * SLOTS;
-  uint64_t* bar_vfree = bars + 8 + 3 * SLOTS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * SLOTS);
+  uint64_t* bar_kfull = bars + 1;          // [2] each
+  uint64_t* bar_vfull = bars + 3;
+  uint64_t* bar_sfull = bars + 5;
+  uint64_t* bar_pfull = bars + 7;
+  uint64_t* bar_pvdone = bars + 9;
+  uint64_t* bar_drain = bars + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // the set-up that touches no global memory runs while the grid before this one finishes
@@ -80,10 +64,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (warp == 4 && lane == 0) {
     mbar_init(bar_q, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_kfull + i, 1);
+      mbar_init(bar_vfull + i, 1);
       mbar_init(bar_sfull + i, 1);
       mbar_init(bar_pvdone + i, 1);
     }
-    for (int i = 0; i < 4 * SLOTS; ++i) mbar_init(bar_kfull + i, 1);   // (and kfree, vfull, vfree)
     mbar_init(bar_drain, 1);
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -115,10 +100,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   // the call's error word: nothing else writes it until a wait of some CTA runs out
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;
-  // loads in the order of their use: K0 V0 K1 V1 .. | K(s + SLOTS) after QK(s), V(s + SLOTS) after PV(s)
+  // loads in the order of their use: K0 V0 K1 V1 | K(s+2) after QK(s), V(s+2) after PV(s)
   auto load = [&](int s, bool is_v) {
-    uint64_t* bar = (is_v ? bar_vfull : bar_kfull) + s % SLOTS;
-    uint8_t* dst = (is_v ? sV : sK) + (s % SLOTS) * SLOT;
+    uint64_t* bar = (is_v ? bar_vfull : bar_kfull) + (s & 1);
+    uint8_t* dst = (is_v ? sV : sK) + (s & 1) * SLOT;
     mbar_arrive_expect_tx(bar, SLOT);
     for (int i = 0; i < NBOX; ++i)
       tma_load_4d(dst + i * HBOX, is_v ? &tm_v : &tm_k, bar, i * 64, hk, steps.key0(s_begin + s), b);
@@ -126,17 +111,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (warp == 4 && lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(bar_pfull + i, 32 * active);
     fence_barrier_init();
-    for (int s = 0; s < min(SLOTS, nsteps); ++s) {
+    for (int s = 0; s < min(2, nsteps); ++s) {
       load(s, false);
       load(s, true);
     }
   }
-  // rows of the tile that no box fills (G does not divide its rows): finite scores for them
-  if (p.RT < Shape::ROWS) {
-    for (int i = threadIdx.x; i < NBOX * Shape::ROWS * 8; i += blockDim.x)
-      if ((i >> 3) % Shape::ROWS >= p.RT) *reinterpret_cast<uint4*>(sQ + i * 16) = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
+  // rows of the tile that no box fills (G does not divide 128): finite scores for them
+  for (int i = threadIdx.x; i < NBOX * (128 - p.RT) * 8; i += blockDim.x) {
+    const int box = i / ((128 - p.RT) * 8), rest = i % ((128 - p.RT) * 8);
+    *reinterpret_cast<uint4*>(sQ + box * QBOX + p.RT * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
   }
+  if (p.RT < 128) fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -149,20 +134,18 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (lane == 0 && nsteps == 0) mbar_wait(bar_q, 0, p.err, kErrWaitDrain);
     if (lane == 0 && nsteps > 0) {
       bool ok = true;
-      int last_k = min(SLOTS, nsteps) - 1, last_v = last_k;
-      for (int s = 0; s + SLOTS < nsteps; ++s) {
-        if (!(ok = mbar_wait(bar_kfree + s % SLOTS, (s / SLOTS) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-        load(last_k = s + SLOTS, false);
-        if (!(ok = mbar_wait(bar_vfree + s % SLOTS, (s / SLOTS) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
-        load(last_v = s + SLOTS, true);
+      int last_k = min(2, nsteps) - 1, last_v = last_k;
+      for (int s = 0; s + 2 < nsteps; ++s) {
+        if (!(ok = mbar_wait(bar_sfull + (s & 1), (s >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        load(last_k = s + 2, false);
+        if (!(ok = mbar_wait(bar_pvdone + (s & 1), (s >> 1) & 1, p.err, kErrWaitLoad, p.wait_ns))) break;
+        load(last_v = s + 2, true);
       }
       if (!ok) {
         // exit path: every issued copy lands before the CTA's shared memory goes away
         mbar_wait(bar_q, 0, p.err, kErrWaitDrain);
-        for (int s = max(0, last_k + 1 - SLOTS); s <= last_k; ++s)
-          mbar_wait(bar_kfull + s % SLOTS, (s / SLOTS) & 1, p.err, kErrWaitDrain);
-        for (int s = max(0, last_v + 1 - SLOTS); s <= last_v; ++s)
-          mbar_wait(bar_vfull + s % SLOTS, (s / SLOTS) & 1, p.err, kErrWaitDrain);
+        for (int s = max(0, last_k - 1); s <= last_k; ++s) mbar_wait(bar_kfull + (s & 1), (s >> 1) & 1, p.err, kErrWaitDrain);
+        for (int s = max(0, last_v - 1); s <= last_v; ++s) mbar_wait(bar_vfull + (s & 1), (s >> 1) & 1, p.err, kErrWaitDrain);
       }
     }
   } else if (warp == 5) {
@@ -178,29 +161,32 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         return done;
       };
       auto issue_qk = [&](int s) {
-        const int slot = s & 1, ring = s % SLOTS;
-        if (!wait(bar_kfull + ring, (s / SLOTS) & 1)) return false;
+        const int slot = s & 1;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
           mma_bf16_ss_warp(mine, tS + slot * 64, desc_at(q_desc, (k >> 2) * QBOX + (k & 3) * 32),
-                           desc_at(k_desc, ring * SLOT + (k >> 2) * HBOX + (k & 3) * 32), IDESC_QK, k > 0);
+                           desc_at(k_desc, slot * SLOT + (k >> 2) * HBOX + (k & 3) * 32), IDESC_QK, k > 0);
         tc_commit_warp(mine, bar_sfull + slot);
-        tc_commit_warp(mine, bar_kfree + ring);
-        return true;
       };
-      bool ok = wait(bar_q, 0) && issue_qk(0) && (nsteps == 1 || issue_qk(1));
+      bool ok = wait(bar_q, 0);
+      for (int s = 0; ok && s < min(2, nsteps); ++s) {
+        if (!(ok = wait(bar_kfull + s, 0))) break;
+        issue_qk(s);
+      }
       for (int s = 0; ok && s < nsteps; ++s) {
         const int slot = s & 1;
         const uint32_t par = (s >> 1) & 1;
-        if (!(ok = wait(bar_pfull + slot, par) && wait(bar_vfull + s % SLOTS, (s / SLOTS) & 1))) break;
+        if (!(ok = wait(bar_pfull + slot, par) && wait(bar_vfull + slot, par))) break;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_bf16_ts_warp(mine, tO, tS + slot * 64 + kk * 8, desc_at(v_desc, (s % SLOTS) * SLOT + kk * 2048), IDESC_PV,
+          mma_bf16_ts_warp(mine, tO, tS + slot * 64 + kk * 8, desc_at(v_desc, slot * SLOT + kk * 2048), IDESC_PV,
                            (s > 0 || kk > 0) ? 1u : 0u);
         tc_commit_warp(mine, bar_pvdone + slot);
-        tc_commit_warp(mine, bar_vfree + s % SLOTS);
-        // QK(s+2) overwrites slot s's P: PV(s) has to have read it
-        if (s + 2 < nsteps) ok = wait(bar_pvdone + slot, par) && issue_qk(s + 2);
+        if (s + 2 < nsteps) {
+          // QK(s+2) overwrites slot s's P: PV(s) has to have read it
+          if (!(ok = wait(bar_pvdone + slot, par) && wait(bar_kfull + slot, ((s + 2) >> 1) & 1))) break;
+          issue_qk(s + 2);
+        }
       }
       // every product issued has completed once bar_drain fires
       tc_commit_warp(mine, bar_drain);
@@ -238,11 +224,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           softmax_half<true, false, HD>(ts, tO + lane_base, bits, p.s2, m_ref, l_sum, s > 0, -1, 0.f, 1.f, drain);
           const WinUnseen unseen(p, seq.L, pa, pb, k0, kStep);
           if (ok && unseen.any(kStep)) {
-            if ((ok = mbar_wait_warp(bar_vfull + s % SLOTS, (s / SLOTS) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) {
+            if ((ok = mbar_wait_warp(bar_vfull + slot, (s >> 1) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) {
               for (int i = row; i < kStep * NBOX * 8; i += 32 * active) {
                 const int r = i / (NBOX * 8), x = i % (NBOX * 8);
                 if ((r >= unseen.a0 && r < unseen.a1) || r >= unseen.b0)
-                  *reinterpret_cast<uint4*>(sV + (s % SLOTS) * SLOT + (x >> 3) * HBOX + r * 128 + (x & 7) * 16) =
+                  *reinterpret_cast<uint4*>(sV + slot * SLOT + (x >> 3) * HBOX + r * 128 + (x & 7) * 16) =
                       make_uint4(0, 0, 0, 0);
               }
               fence_proxy_async_smem();
@@ -384,11 +370,12 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   }
 }
 
-template <int HD, bool FEW>
+template <int HD>
 cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
-  auto kern = window_fwd_kernel<HD, FEW>;
+  auto kern = window_fwd_kernel<HD>;
   // at least ~100 KB, so that at most two CTAs (512 TMEM columns) share an SM
-  constexpr size_t need = FwdShape<HD, FEW>::SMEM, smem = need < 100 * 1024 ? 100 * 1024 : need;
+  constexpr size_t need = (HD / 64) * (128 * 128 + 4 * kStep * 128) + 256 + 1024;
+  const size_t smem = need < 100 * 1024 ? 100 * 1024 : need;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
@@ -402,8 +389,7 @@ cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_window_fwd(int hd, const WinMaps& m, const WinParams& p, cudaStream_t st) {
-  if (p.few) return hd == 128 ? launch_t<128, true>(m, p, st) : launch_t<64, true>(m, p, st);
-  return hd == 128 ? launch_t<128, false>(m, p, st) : launch_t<64, false>(m, p, st);
+  return hd == 128 ? launch_t<128>(m, p, st) : launch_t<64>(m, p, st);
 }
 
 }  // namespace solb200
