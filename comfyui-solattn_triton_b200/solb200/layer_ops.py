@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 from contextlib import nullcontext
-from ctypes import c_int32, c_int64
+from ctypes import c_float, c_int32, c_int64
 from types import SimpleNamespace
 
 import torch
@@ -84,9 +84,33 @@ def _bthd(t, name, dtype, device, shape=None):
         _refuse(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
 
 
+def _numbers(**named):
+    # (a tensor's value could change under a plan kept for it)
+    for name, x in named.items():
+        if torch.is_tensor(x):
+            _refuse(f"{name} must be a number, not a tensor")
+
+
+def _fresh(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _strides(t):
     s = t.stride()
     return I64x3(s[0], s[1], s[2])
+
+
+def _dense(B, T, H, D):
+    return I64x3(T * H * D, H * D, D)
+
+
+def _readable(t, dense, broadcast):
+    """(tensor, strides) of `t` as the kernels can read it; `dense`: the strides of a packed one
+    (head_dim is a multiple of 16 bytes)."""
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t, dense
+    t = _rows16(t, broadcast)
+    return t, _strides(t)
 
 
 def _in_place(t, broadcast):
@@ -100,6 +124,7 @@ def _in_place(t, broadcast):
 
 
 def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
+    _numbers(eps=eps, interleaved=interleaved)
     if q.dtype not in DTYPES:
         _refuse(f"q must be bfloat16, float16 or float32 (got {q.dtype})")
     _bthd(q, "q", q.dtype, q.device)
@@ -131,8 +156,10 @@ def _rope_plan(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
     if B and T and H:
         check(lib().solb200_qk_norm_rope_backward_workspace(B, T, H, Hk, D, ctypes.byref(n)), "workspace")
     return SimpleNamespace(
-        place=(B, T, H, Hk, D, R, DTYPES[q.dtype], float(eps), int(bool(interleaved))), empty=not (B and T and H),
+        place=(c_int64(B), c_int64(T), c_int64(H), c_int64(Hk), c_int64(D), c_int64(R), c_int32(DTYPES[q.dtype]),
+               c_float(eps), c_int32(bool(interleaved))), empty=not (B and T and H),
         wtype=DTYPES[q_weight.dtype], qs=_strides(q), ks=_strides(k), backward_bytes=n.value,
+        dense_q=_dense(B, T, H, D), dense_k=_dense(B, T, Hk, D),
         ts=I64x2(0, cos.stride(0)) if cos.dim() == 2 else I64x2(cos.stride(0), cos.stride(1)),
         in_place=(_in_place(q, True) and _in_place(k, True) and _in_place(cos, True) and cos.stride() == sin.stride()
                   and q_weight.is_contiguous() and k_weight.is_contiguous()))
@@ -156,8 +183,7 @@ def _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
 
 def _rope_forward(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
     plan, q, k, wq, wk, cos, sin = _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
-    B, T, H, Hk, D = plan.place[:5]
-    q_out, k_out = q.new_empty((B, T, H, D)), q.new_empty((B, T, Hk, D))
+    q_out, k_out = _fresh(q), _fresh(k)
     if not plan.empty:
         index = q.get_device()
         with _on(index):
@@ -176,17 +202,17 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *,
     for g, x, name in ((dq_out, q, "dq_out"), (dk_out, k, "dk_out")):
         if g.shape != x.shape or g.dtype != x.dtype or g.get_device() != x.get_device():
             _bthd(g, name, x.dtype, x.device, x.shape)
-    dq_out, dk_out = _rows16(dq_out, True), _rows16(dk_out, True)
-    B, T, H, Hk, D = plan.place[:5]
-    dq, dk = q.new_empty((B, T, H, D)), q.new_empty((B, T, Hk, D))
+    dq_out, dqs = _readable(dq_out, plan.dense_q, True)
+    dk_out, dks = _readable(dk_out, plan.dense_k, True)
+    dq, dk = _fresh(q), _fresh(k)
     if plan.empty:
         return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk)
-    dwq, dwk = wq.new_empty(D), wq.new_empty(D)
+    dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
     index = q.get_device()
     with _on(index):
         ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=q.device)
         rc = lib().solb200_qk_norm_rope_backward(
-            dq_out.data_ptr(), _strides(dq_out), dk_out.data_ptr(), _strides(dk_out), q.data_ptr(), plan.qs,
+            dq_out.data_ptr(), dqs, dk_out.data_ptr(), dks, q.data_ptr(), plan.qs,
             k.data_ptr(), plan.ks, wq.data_ptr(), wk.data_ptr(), plan.wtype, cos.data_ptr(), sin.data_ptr(), plan.ts,
             dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), *plan.place, ws.data_ptr(),
             plan.backward_bytes, _raw_stream(index))
@@ -235,6 +261,7 @@ def _bound(x, name):
 
 
 def _window_plan(q, k, v, left, right, sinks, scale):
+    _numbers(left=left, right=right, sinks=sinks, scale=scale)
     _bthd(q, "q", torch.bfloat16, q.device)
     _bthd(k, "k", torch.bfloat16, q.device)
     _bthd(v, "v", torch.bfloat16, q.device, k.shape)
@@ -258,8 +285,9 @@ def _window_plan(q, k, v, left, right, sinks, scale):
         for backward in (0, 1):
             check(lib().solb200_window_attn_workspace(B, Tq, Tk, H, Hk, D, *bounds, backward,
                                                       ctypes.byref(n[backward])), "window_attn workspace")
-    return SimpleNamespace(place=(B, Tq, Tk, H, Hk, D, *bounds, scale), empty=empty, bytes=n[0].value,
+    return SimpleNamespace(place=(*map(c_int64, (B, Tq, Tk, H, Hk, D, *bounds)), c_float(scale)), empty=empty, bytes=n[0].value,
                            backward_bytes=n[1].value, qs=_strides(q), ks=_strides(k), vs=_strides(v),
+                           dense_q=_dense(B, Tq, H, D),
                            in_place=_in_place(q, False) and _in_place(k, False) and _in_place(v, False))
 
 
@@ -309,13 +337,12 @@ def _workspace(nbytes, q, index, stream):
 
 def _window_forward(q, k, v, left, right, sinks, scale, lengths, offsets, want_lse):
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
-    B, Tq, _, H, _, D = plan.place[:6]
+    B, Tq, H, _ = q.shape
     if plan.empty:      # no queries, or no keys for them to see
-        return (q.new_zeros((B, Tq, H, D)),
-                torch.full((B, H, Tq), -torch.inf, device=q.device) if want_lse else None)
+        return (q.new_zeros(q.shape), torch.full((B, H, Tq), -torch.inf, device=q.device) if want_lse else None)
     index = q.get_device()
     with _on(index):
-        out = q.new_empty((B, Tq, H, D))
+        out = _fresh(q)
         lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
         stream = _raw_stream(index)
         ws = _workspace(plan.bytes, q, index, stream)
@@ -335,7 +362,7 @@ def window_attn_backward(dout, q, k, v, out, lse, *, left=None, right=0, sinks=0
     its log-sum-exp (``return_lse``), with the same bounds. Sums are in a fixed order. ``q`` and
     ``dout`` have to be finite in every row, the rows of queries that see nothing included."""
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
-    B, Tq, Tk, H, Hk, D = plan.place[:6]
+    B, Tq, H, _ = q.shape
     for t, name in ((dout, "dout"), (out, "out")):
         if t.shape != q.shape or t.dtype != q.dtype or t.get_device() != q.get_device():
             _bthd(t, name, q.dtype, q.device, q.shape)
@@ -343,15 +370,17 @@ def window_attn_backward(dout, q, k, v, out, lse, *, left=None, right=0, sinks=0
         _refuse(f"lse must be float32 [{B}, {H}, {Tq}] on {q.device}")
     if plan.empty:
         return tuple(t.new_zeros(t.shape) for t in (q, k, v))
-    dout, out, lse = _rows16(dout, False), _rows16(out, False), lse.contiguous()
+    dout, dos = _readable(dout, plan.dense_q, False)
+    out, outs = _readable(out, plan.dense_q, False)
+    lse = lse.contiguous()
     index = q.get_device()
     with _on(index):
-        dq, dk, dv = q.new_empty((B, Tq, H, D)), q.new_empty((B, Tk, Hk, D)), q.new_empty((B, Tk, Hk, D))
+        dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
         ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=q.device)
         stream = _raw_stream(index)
         rc = lib().solb200_window_attn_backward(
-            dout.data_ptr(), _strides(dout), q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, v.data_ptr(), plan.vs,
-            out.data_ptr(), _strides(out), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            dout.data_ptr(), dos, q.data_ptr(), plan.qs, k.data_ptr(), plan.ks, v.data_ptr(), plan.vs,
+            out.data_ptr(), outs, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             _ptr(lengths), _ptr(offsets), *plan.place, ws.data_ptr(), plan.backward_bytes, stream)
         if rc:
             check(rc, "window_attn_backward")

@@ -69,3 +69,13 @@ def test_host_tensors_are_refused():
         solb200.window_attn(q, q, q)
     with pytest.raises(RuntimeError, match="CUDA"):
         solb200.window_attn_backward(q, q, q, q, q, torch.zeros(1, 2, 8))
+
+
+def test_options_are_numbers_not_tensors():
+    q = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    w, t = torch.ones(64), torch.zeros(8, 32)
+    with pytest.raises(RuntimeError, match="eps must be a number"):
+        solb200.qk_norm_rope(q, q, w, w, t, t, eps=torch.tensor(1e-6))
+    for name in ("left", "right", "sinks", "scale"):
+        with pytest.raises(RuntimeError, match=f"{name} must be a number"):
+            solb200.window_attn(q, q, q, **{name: torch.tensor(4)})
