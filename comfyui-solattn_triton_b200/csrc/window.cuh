@@ -115,6 +115,17 @@ struct WinUnseen {
   __device__ bool any(int n) const { return a1 > a0 || b0 < n; }
 };
 
+// Of the TPT tokens from t0 on, those outside [t0, t1) (counted from t0) see nothing: they come
+// before the first key by more than the right bound, or past the last one by more than the left.
+struct WinBlind {
+  int t0, t1;
+  __device__ WinBlind(const WinParams& p, const WinSeq& seq, int first) {
+    t0 = p.right < 0 ? 0 : clamp_to(-p.right - seq.off - first, 0, p.TPT);
+    t1 = p.left < 0 || p.sinks > 0 ? p.TPT : clamp_to(seq.L + p.left - seq.off - first, 0, p.TPT);
+  }
+  __device__ bool any(const WinParams& p) const { return t0 > 0 || t1 < p.TPT; }
+};
+
 struct WinMaps {
   CUtensorMap q, k, v, o;        // o: the forward's output, the gradient's dq
   CUtensorMap dout, dk, dv;      // gradient

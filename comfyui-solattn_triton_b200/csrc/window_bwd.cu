@@ -443,6 +443,21 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (full) load_dp<false>(tdp, mask, dp);
       else load_dp<true>(tdp, mask, dp);
       store_cols(tdp, pr);
+      // queries and dO of tokens that see nothing may hold anything: their rows are zeroed before the
+      // sums, each column group its own quarter (S(i) and dP(i), which read them too, are complete)
+      const WinBlind blind(p, seq, t0);
+      if (!full && blind.any(p)) {
+        if (!(ok = mbar_wait_warp(bar_q + i % 3, (i / 3) & 1, p.err, kErrWaitSoftmax, p.wait_ns))) break;
+        for (int c = threadIdx.x & 127; c < 32 * NBOX * 8; c += 128) {
+          const int r = c0 + c / (NBOX * 8), x = c % (NBOX * 8);
+          if (r < blind.t0 * p.G || r >= blind.t1 * p.G) {
+            const uint32_t at = (x >> 3) * kBox + r * 128 + (x & 7) * 16;
+            *reinterpret_cast<uint4*>(sG + st * TILE + at) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(sQ + (i % 3) * TILE + at) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(bar_p + wg);

@@ -360,7 +360,7 @@ def window_attn_backward(dout, q, k, v, out, lse, *, left=None, right=0, sinks=0
                          offsets=None):
     """(dq, dk, dv) from the gradient of ``window_attn``'s output, its inputs, its output and
     its log-sum-exp (``return_lse``), with the same bounds. Sums are in a fixed order. ``q`` and
-    ``dout`` have to be finite in every row, the rows of queries that see nothing included."""
+    ``dout`` of queries that see nothing may hold anything (their dq is zero)."""
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
     B, Tq, H, _ = q.shape
     for t, name in ((dout, "dout"), (out, "out")):

@@ -330,7 +330,8 @@ SOLB200_API int32_t solb200_window_attn(const void* q, const int64_t* q_strides,
 
 /* Gradient of solb200_window_attn: dq, dk, dv (dense bf16) from dout (strided like q) and the
  * forward's inputs, out and lse, with its bounds. Keys that no query sees get zeros. Sums are
- * in a fixed order: the same bits every time. q and dout have to be finite in every row. */
+ * in a fixed order: the same bits every time. q and dout of queries that see nothing may hold
+ * anything. */
 SOLB200_API int32_t solb200_window_attn_backward(
     const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides, const void* k,
     const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides,

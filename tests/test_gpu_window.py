@@ -246,6 +246,31 @@ def test_keys_outside_every_window_are_not_used(cuda_device, Tq):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("Tq,Hk,D", [(1, 2, 64), (100, 4, 64), (300, 2, 128), (300, 4, 64), (700, 1, 128)])
+@pytest.mark.parametrize("ends", ["before", "past"])
+def test_queries_that_see_nothing_are_not_used(cuda_device, Tq, Hk, D, ends):
+    """NaN and infinities in the queries, and in their outputs' gradients, of padding before a
+    sequence's first key or past its last window leave the gradients of all keys as they were."""
+    q, k, v = (t.cuda() for t in _inputs(4, Tq, 700, 4, Hk, D, seed=31))
+    lengths = [0, 1, Tq // 3, Tq]
+    offsets = [n - Tq for n in lengths] if ends == "before" else [0] * 4
+    left = None if ends == "before" else 20
+    how = dict(left=left, lengths=torch.tensor(lengths, dtype=torch.int32).cuda(),
+               offsets=torch.tensor(offsets, dtype=torch.int32).cuda())
+    clean = solb200.window_attn(q, k, v, return_lse=True, **how)
+    dout = torch.randn_like(q)
+    blind = torch.isneginf(clean[1]).transpose(1, 2)
+    assert blind[0].all() and blind[1:].any() and (Tq == 1 or not blind[1:].all())
+    grads = solb200.window_attn_backward(dout, q, k, v, *clean, **how)
+    q2 = torch.where(blind[..., None], torch.tensor(float("nan"), device="cuda", dtype=q.dtype), q)
+    dout2 = torch.where(blind[..., None], torch.tensor(float("inf"), device="cuda", dtype=q.dtype), dout)
+    dirty = solb200.window_attn(q2, k, v, return_lse=True, **how)
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for a, b in zip(grads, solb200.window_attn_backward(dout2, q2, k, v, *dirty, **how)):
+        assert torch.equal(a, b)
+    assert not grads[0][blind].any()
+
+
 def test_agrees_with_the_dense_kernel(cuda_device):
     """No bounds: the dense call's attention, up to both calls' roundings."""
     q, k, v = _inputs(1, 500, 900, 3, 3, 128, seed=3)
