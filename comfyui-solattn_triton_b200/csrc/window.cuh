@@ -31,8 +31,8 @@ struct WinParams {
   const float* lse_in;      // [B, H, Tq]
   const __nv_bfloat16 *o_in, *do_in;
   int64_t os[3], dos[3];    // strides {batch, token, head}
-  float* rows_lse;          // [B, Hk, nqt, 128] lse * log2(e) by tile row (+inf: nothing seen, or no row)
-  float* rows_delta;        // [B, Hk, nqt, 128] sum(dO * O) by tile row
+  float* rows_lse;          // [B, Hk, nqt, 128] -lse * log2(e) by tile row (-inf: nothing seen, or no row)
+  float* rows_delta;        // [B, Hk, nqt, 128] -sum(dO * O) by tile row
   int nkt;                  // key tiles of 128
   int split_q, split_k;     // parts of a query tile's key steps (dq) and of a key tile's query tiles (dk, dv)
   float* part_dq;           // [split_q, B, Tq, H, D] if split_q > 1

@@ -24,12 +24,12 @@
 // Where the tiles are too few to fill the GPU, a tile's walk is divided over split_q (split_k) CTAs,
 // which write their sums in 32 bits; window_grad_join_kernel adds them up in order.
 //
-// window_rows_kernel comes first: -delta and -lse * log2(e) laid out by query tile, -inf for rows
-// that see nothing and for the tile's rows past the last token, which makes their P zero. Its
-// delta carries the rounding of O to bf16, which counts where a row sees few keys (one key: dS
-// is zero). For tiles of up to kFewSteps steps window_dq_kernel therefore forms delta =
-// sum(P dP) / sum(P) in 32 bits first (sum(P) is 1 up to the rounding of lse), and leaves it for
-// window_dkv_kernel.
+// window_dq_kernel comes first and leaves -delta and -lse * log2(e) of its rows, by query tile, for
+// window_dkv_kernel: -inf for rows that see nothing and for the tile's rows past the last token, which
+// makes their P zero. (As a kernel of their own they took 26 us of the 1103 that the forward and the gradient took at the sizes above.)
+// delta = sum(dO * O) carries the rounding of O to bf16, which counts where a row sees few keys (one
+// key: dS is zero). For tiles of up to kFewSteps steps the kernel therefore forms delta =
+// sum(P dP) / sum(P) in 32 bits before dS (sum(P) is 1 up to the rounding of lse).
 #include "fwd_common.cuh"
 #include "window.cuh"
 
@@ -148,39 +148,51 @@ __global__ void __launch_bounds__(256) window_grad_join_kernel(const __grid_cons
                                                   pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
 }
 
-// One row per HD / 8 lanes.
+// A query tile's row numbers, from the forward's output and log-sum-exp and from dO: -lse * log2(e)
+// (-inf for rows that see nothing and past the tile's tokens) and -delta, into shared memory. One row
+// per HD / 8 of the softmax threads; the loads land while the first tiles and scores are on their way.
 template <int HD>
-__global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WinParams p) {
-  pdl_begin();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;   // the call's error word
-  constexpr int GL = HD / 8, PER_TILE = kTile * GL / 256;   // CTAs per query tile
-  const int lg = threadIdx.x % GL;
-  const int tile = blockIdx.x / PER_TILE, row = (blockIdx.x % PER_TILE) * (256 / GL) + threadIdx.x / GL;
-  const int64_t slot = (int64_t)tile * kTile + row;         // [B, Hk, nqt, 128]
-  const DivMod by_tile(tile, p.nqt), by_hk(by_tile.quot, p.Hk), by_g(row, p.G);
-  const int hk = by_hk.rem, b = by_hk.quot;
-  const int tok = by_tile.rem * p.TPT + by_g.quot, h = hk * p.G + by_g.rem;
-  const bool live = row < p.RT && tok < p.Tq;
-  float d = 0.f, neg = -INFINITY;
-  if (live) {
-    const uint4 wo = __ldg(reinterpret_cast<const uint4*>(p.o_in + b * p.os[0] + tok * p.os[1] + h * p.os[2]) + lg);
-    const uint4 wd = __ldg(reinterpret_cast<const uint4*>(p.do_in + b * p.dos[0] + tok * p.dos[1] + h * p.dos[2]) + lg);
-    const uint32_t o[4] = {wo.x, wo.y, wo.z, wo.w}, g[4] = {wd.x, wd.y, wd.z, wd.w};
+struct RowNumbers {
+  static constexpr int GL = HD / 8, AT_ONCE = kSoftmax / GL, PASSES = kTile / AT_ONCE;
+  uint4 wo[PASSES], wd[PASSES];
+  float lse[PASSES];
+
+  __device__ __forceinline__ RowNumbers(const WinParams& p, int b, int hk, int t0, int rows) {
+    const int lg = threadIdx.x % GL;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      d = fmaf(__uint_as_float(o[i] << 16), __uint_as_float(g[i] << 16), d);
-      d = fmaf(__uint_as_float(o[i] & 0xffff0000u), __uint_as_float(g[i] & 0xffff0000u), d);
+    for (int i = 0; i < PASSES; ++i) {
+      const int row = i * AT_ONCE + threadIdx.x / GL;
+      const DivMod by_g(row, p.G);
+      const int tok = t0 + by_g.quot, h = hk * p.G + by_g.rem;
+      wo[i] = wd[i] = make_uint4(0, 0, 0, 0);
+      lse[i] = -INFINITY;
+      if (row < rows) {
+        wo[i] = __ldg(reinterpret_cast<const uint4*>(p.o_in + b * p.os[0] + tok * p.os[1] + h * p.os[2]) + lg);
+        wd[i] = __ldg(reinterpret_cast<const uint4*>(p.do_in + b * p.dos[0] + tok * p.dos[1] + h * p.dos[2]) + lg);
+        lse[i] = __ldg(p.lse_in + ((int64_t)b * p.H + h) * p.Tq + tok);
+      }
     }
-    const float lse = __ldg(p.lse_in + ((int64_t)b * p.H + h) * p.Tq + tok);
-    if (lse != -INFINITY) neg = -lse * 1.4426950408889634f;
   }
+  __device__ __forceinline__ void store(float* neg_lse, float* neg_delta) {
 #pragma unroll
-  for (int o = GL / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  if (lg == 0) {
-    p.rows_lse[slot] = neg;
-    p.rows_delta[slot] = neg == -INFINITY ? 0.f : -d;
+    for (int i = 0; i < PASSES; ++i) {
+      const uint32_t o[4] = {wo[i].x, wo[i].y, wo[i].z, wo[i].w}, g[4] = {wd[i].x, wd[i].y, wd[i].z, wd[i].w};
+      float d = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        d = fmaf(__uint_as_float(o[j] << 16), __uint_as_float(g[j] << 16), d);
+        d = fmaf(__uint_as_float(o[j] & 0xffff0000u), __uint_as_float(g[j] & 0xffff0000u), d);
+      }
+#pragma unroll
+      for (int x = GL / 2; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+      const int row = i * AT_ONCE + threadIdx.x / GL;
+      if (threadIdx.x % GL == 0) {
+        neg_lse[row] = lse[i] == -INFINITY ? -INFINITY : -lse[i] * 1.4426950408889634f;
+        neg_delta[row] = lse[i] == -INFINITY ? 0.f : -d;
+      }
+    }
   }
-}
+};
 
 // 32 columns of P for one TMEM lane: 2^(s * s2 - lse * log2(e)), s the raw scores in r. `nl(i)` gives
 // -lse * log2(e) of columns 4 i .. 4 i + 3 (where a lane is a query row, the same for all).
@@ -531,6 +543,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* bar_drain = bars + 21;
   uint64_t* bar_taken = bars + 22;       // dP(i) is in the softmax threads' registers
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  float* sRow = reinterpret_cast<float*>(bars + 24);   // -lse * log2(e) [128], -delta [128]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // the set-up that touches no global memory runs while the grid before this one finishes
@@ -570,10 +583,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       tma_load_4d(sG + x * kBox, &tm_do, bar_q, x * 64, hk * p.G, t0, b);
     }
   }
+  const int rows = ntok * p.G;
+  RowNumbers<HD> numbers(p, b, hk, t0, warp < kSoftmax / 32 ? rows : 0);
   const WinSeq seq(p, b);
   const int64_t pa = seq.off + t0, pb = pa + ntok - 1;
   const WinSteps<kTile> steps(p, seq.L, pa, pb);
-  const int rows = ntok * p.G;
   // passes over steps: with 2 .. kFewSteps steps, one pass for delta before the one for dS (a
   // single step has all of a row's P and dP at hand)
   const bool few = steps.n <= kFewSteps;   // (not divided: the first part takes all)
@@ -604,6 +618,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     if (n > 2) load_k(2);
   }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;   // the call's error word
   if (p.RT < kTile && n > 0) {
     zero_rows<HD>(sQ, p.RT, threadIdx.x, kThreads);
     zero_rows<HD>(sG, p.RT, threadIdx.x, kThreads);
@@ -684,8 +699,14 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     // every row of the tile sees the keys [full_lo, full_hi), and the sinks before full_hi
     const int full_hi = win_hi(p, seq.L, pa), full_lo = win_lo(p, pb);
     const int64_t slot = (((int64_t)b * p.Hk + hk) * p.nqt + qt) * kTile + row;
-    const float neg = p.rows_lse[slot];
-    float ndelta = p.rows_delta[slot];
+    numbers.store(sRow, sRow + kTile);
+    named_bar_sync(1, kSoftmax);
+    const float neg = sRow[row];
+    float ndelta = sRow[kTile + row];
+    if (split == 0 && wg == 0) {
+      p.rows_lse[slot] = neg;
+      p.rows_delta[slot] = ndelta;
+    }
     float sum = 0.f, psum = 0.f;   // of P dP and P over this thread's columns, for delta
     bool owes = few && n > 0;
     // delta of the row from its four threads' parts, for this kernel and for window_dkv_kernel; the
@@ -793,15 +814,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 template <int HD>
 cudaError_t launch_t(const WinMaps& m, const WinParams& p, cudaStream_t st) {
   constexpr size_t TILE = (HD / 64) * kBox;
-  constexpr size_t smem_kv = 7 * TILE + 2048 + 256 + 768, smem_q = 7 * TILE + 256 + 1024;
+  constexpr size_t smem_kv = 7 * TILE + 2048 + 256 + 768, smem_q = 7 * TILE + 256 + 1024 + 1024;
   static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
   cudaError_t e = allow_smem(window_dkv_kernel<HD>, smem_kv, allowed_kv);
   if (e == cudaSuccess) e = allow_smem(window_dq_kernel<HD>, smem_q, allowed_q);
   if (e != cudaSuccess) return e;
-  const int64_t slots = (int64_t)p.B * p.Hk * p.nqt * kTile;
-  e = launch_pdl(window_rows_kernel<HD>, dim3((unsigned)(slots * (HD / 8) / 256)), dim3(256), 0, st, p);
-  if (e != cudaSuccess) return e;
-  // window_dq_kernel leaves refined deltas for window_dkv_kernel
+  // window_dq_kernel leaves the rows' numbers for window_dkv_kernel
   const int64_t heads = (int64_t)p.B * p.Hk;
   e = launch_pdl(window_dq_kernel<HD>, dim3((unsigned)(heads * p.nqt * p.split_q)), dim3(kThreads), smem_q, st, m.q, m.k,
                  m.v, m.dout, m.o, p);
