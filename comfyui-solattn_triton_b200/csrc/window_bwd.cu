@@ -16,17 +16,18 @@
 // columns; 256 threads took 616 us where these took 566, in the first form of window_dkv_kernel), one
 // TMA warp, one MMA warp, one CTA per SM.
 //
-// Measured on a B200, 4 x 4096 tokens x 24 heads x 128, about 1000 keys a row: window_dq_kernel 373 us,
-// window_dkv_kernel 489 us, 0.91 PFLOP/s of products executed each. An iteration takes 2700 and
-// 3200 cycles against 1536 and 2048 of products: the softmax threads are busy for 2400 and 2700 of
-// them, and only what the barriers allow runs at the same time.
+// Measured on a B200, 4 x 4096 tokens x 24 heads x 128, about 1000 keys a row: window_dq_kernel 370 us,
+// window_dkv_kernel 472 us, 0.90 and 0.94 PFLOP/s of products executed. An iteration takes 2400 and
+// 3300 cycles against 1536 and 2048 of products: the softmax threads are busy for most of them, and
+// only what the barriers allow runs at the same time.
 //
 // Where the tiles are too few to fill the GPU, a tile's walk is divided over split_q (split_k) CTAs,
 // which write their sums in 32 bits; window_grad_join_kernel adds them up in order.
 //
 // window_dq_kernel comes first and leaves -delta and -lse * log2(e) of its rows, by query tile, for
 // window_dkv_kernel: -inf for rows that see nothing and for the tile's rows past the last token, which
-// makes their P zero. (As a kernel of their own they took 26 us of the 1103 that the forward and the gradient took at the sizes above.)
+// makes their P zero. (As a kernel of their own they took 26 us of the 1103 that the forward and the
+// gradient took at the sizes above.)
 // delta = sum(dO * O) carries the rounding of O to bf16, which counts where a row sees few keys (one
 // key: dS is zero). For tiles of up to kFewSteps steps the kernel therefore forms delta =
 // sum(P dP) / sum(P) in 32 bits before dS (sum(P) is 1 up to the rounding of lse).
