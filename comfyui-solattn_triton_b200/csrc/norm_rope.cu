@@ -585,8 +585,15 @@ int norm_rope_backward_ctas(int64_t B, int64_t T, int64_t H, int64_t Hk, int D) 
   RopeParams p{};
   p.B = (int)B; p.T = (int)T; p.D = D;
   p.t[0].heads = (int)H; p.t[1].heads = (int)Hk;
-  plan_ctas(p, rows_in_flight(true), kMostCtas);   // (of every type, the one with the most CTAs)
-  return p.ctas[0] + p.ctas[1];
+  // the more of the two run lengths' plans (the element type is not known here): shorter runs take more
+  // CTAs, but past kMostCtas the tensors' shares are rounded down and may add up to one less
+  int most = 0;
+  for (const bool wide : {false, true}) {
+    plan_ctas(p, rows_in_flight(wide), kMostCtas);
+    const int ctas = p.ctas[0] + p.ctas[1];
+    most = ctas > most ? ctas : most;
+  }
+  return most;
 }
 
 cudaError_t launch_norm_rope_backward(RopeParams p, int dtype, int wdtype, bool interleaved, cudaStream_t st) {

@@ -35,7 +35,8 @@ struct RopeParams {
 
 cudaError_t launch_norm_rope(RopeParams p, int dtype, int wdtype, bool interleaved, cudaStream_t st);
 cudaError_t launch_norm_rope_backward(RopeParams p, int dtype, int wdtype, bool interleaved, cudaStream_t st);
-// CTAs of the backward pass for this geometry (the lines of RopeParams::partial)
+// Most CTAs that the backward pass of any element type takes for this geometry (the lines of
+// RopeParams::partial)
 int norm_rope_backward_ctas(int64_t B, int64_t T, int64_t H, int64_t Hk, int D);
 
 }  // namespace solb200

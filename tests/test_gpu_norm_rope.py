@@ -244,3 +244,27 @@ def test_refusals(cuda_device):
         solb200.qk_norm_rope(q, k, wq, wk, cos[..., :4], sin[..., :4], interleaved=False)
     with pytest.raises(RuntimeError, match="solb200"):
         solb200.qk_norm_rope_backward(q[:, :3], k, q, k, wq, wk, cos, sin)
+
+
+@pytest.mark.parametrize("T,H,Hk,D", [(710, 32, 8, 128), (709, 32, 8, 128), (1418, 32, 8, 64), (354, 32, 8, 256)])
+def test_gradient_stays_in_its_workspace(cuda_device, T, H, Hk, D):
+    """Sizes at which 16-bit types take every CTA of the GPU: nothing behind the workspace's bytes changes."""
+    import ctypes
+    from ctypes import c_int32, c_int64
+    from solb200._lib import I64x2, I64x3, lib
+    q, k, wq, wk, cos, sin = (t.cuda() for t in _inputs(1, T, H, Hk, D, D, torch.bfloat16, per_batch=False, seed=8))
+    g = torch.Generator().manual_seed(9)
+    dys = [torch.randn(t.shape, generator=g).bfloat16().cuda() for t in (q, k)]
+    want = solb200.qk_norm_rope_backward(*dys, q, k, wq, wk, cos, sin)
+    n = c_int64(0)
+    assert lib().solb200_qk_norm_rope_backward_workspace(1, T, H, Hk, D, ctypes.byref(n)) == 0
+    ws = torch.full((n.value + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    got = [torch.empty_like(t) for t in (q, k, wq, wk)]
+    st = lambda t: I64x3(*t.stride()[:3])
+    rc = lib().solb200_qk_norm_rope_backward(
+        dys[0].data_ptr(), st(q), dys[1].data_ptr(), st(k), q.data_ptr(), st(q), k.data_ptr(), st(k), wq.data_ptr(),
+        wk.data_ptr(), 0, cos.data_ptr(), sin.data_ptr(), I64x2(0, D // 2), *(t.data_ptr() for t in got), 1, T, H, Hk, D,
+        D, c_int32(0), 1e-6, c_int32(1), ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert (ws[n.value:] == 0xA5).all()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -79,3 +79,24 @@ def test_options_are_numbers_not_tensors():
     for name in ("left", "right", "sinks", "scale"):
         with pytest.raises(RuntimeError, match=f"{name} must be a number"):
             solb200.window_attn(q, q, q, **{name: torch.tensor(4)})
+
+
+def _rope_lines(rows, per, most=148 * 3):
+    """CTAs of the rotation's gradient: one run per warp while they last, else a share of `most`."""
+    want = [-(-r // per) for r in rows]
+    if sum(want) > most:
+        want = [min(w, max(1, most * r // sum(rows))) for w, r in zip(want, rows)]
+    return sum(want)
+
+
+@pytest.mark.parametrize("D,lanes", [(64, 8), (128, 16), (256, 32)])
+def test_rope_gradient_workspace_holds_every_types_lines(D, lanes):
+    """One line of D sums per CTA, whether the element type takes 4 rows a run (16 bits) or 2 (32)."""
+    n, short = ctypes.c_int64(-1), []
+    for H, Hk in ((32, 8), (16, 4), (8, 2), (32, 4), (28, 4), (64, 8), (40, 40), (24, 24), (15, 5), (1, 1)):
+        for T in range(1, 6000):
+            assert _lib.lib().solb200_qk_norm_rope_backward_workspace(1, T, H, Hk, D, ctypes.byref(n)) == 0
+            need = max(_rope_lines((T * H, T * Hk), 32 // lanes * rows * 8) for rows in (4, 2))
+            if n.value < need * D * 4:
+                short.append((T, H, Hk))
+    assert not short
