@@ -678,6 +678,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       bool ok = wait(bar_q, 0) && issue_s(0) && issue_dp(0) && (n == 1 || issue_s(1));
       for (int i = 0; ok && i < n; ++i) {
         if (i + 1 < n && !(ok = wait(bar_taken, i & 1) && issue_dp(i + 1))) break;
+        // the first product overwrites the columns through which all four groups exchanged their sums for
+        // delta (refine): each has read them once its dS is stored
+        if (few && i == npre)
+          for (int c = 0; ok && c < 4; ++c) ok = wait(bar_ds + (i & 1) * 4 + c, (i >> 1) & 1);
         for (int c = 0; ok && c < 4; ++c)
           if ((ok = wait(bar_ds + (i & 1) * 4 + c, (i >> 1) & 1)) && i >= npre)
             mma_sum_quarter<HD>(mine, tDQ, tS + (i & 1) * 128, desc_at(k_sum, (i % 3) * TILE), c, i == npre);
@@ -711,7 +715,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     float sum = 0.f, psum = 0.f;   // of P dP and P over this thread's columns, for delta
     bool owes = few && n > 0;
     // delta of the row from its four threads' parts, for this kernel and for window_dkv_kernel; the
-    // parts meet in dQ's columns, which the first dQ product overwrites later
+    // parts meet in dQ's columns: the first dQ product waits until every group's dS is stored, after this
     auto refine = [&]() {
       owes = false;
       tmem_st1(tDQ + lane_base + wg, __float_as_uint(sum));

@@ -436,3 +436,24 @@ def test_c_abi_refusals(cuda_device):
     assert call(outp=None) == 2 and call(wsp=None) == 3 and call(n=256) == 3 and call(wsp=ws.data_ptr() + 4) == 2
     assert call(lens=ws.data_ptr() + 2) == 2 and call(scale=-1.0) == 1
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T,H,Hk,D,how", [(128, 8, 8, 128, {}), (100, 6, 2, 64, {}), (97, 4, 2, 128, dict(right=None)),
+                                          (128, 40, 8, 64, dict(left=90, sinks=3))])
+def test_gradient_of_sequences_of_one_key_step(cuda_device, T, H, Hk, D, how):
+    """Query tiles whose keys lie in one step, many on the GPU at a time: copies of a sequence all give
+    the same bits, every time, and those of the definition up to its bounds. (The row sums behind delta
+    are exchanged where the first product of dQ goes.)"""
+    copies = 64
+    one = _inputs(1, T, T, H, Hk, D, seed=41)
+    do = torch.randn(one[0].shape, generator=torch.Generator().manual_seed(42)).bfloat16()
+    q, k, v, dout = (t.cuda().repeat(copies, 1, 1, 1) for t in (*one, do))
+    out, lse = solb200.window_attn(q, k, v, return_lse=True, **how)
+    first = None
+    for _ in range(20):
+        got = solb200.window_attn_backward(dout, q, k, v, out, lse, **how)
+        first = first or [t[:1].clone() for t in got]
+        assert all(torch.equal(t, f.expand_as(t)) for t, f in zip(got, first))
+    _, _, _, _, want, bounds = _definition(*one, dout=do, **how)
+    for a, w, bd, name in zip(first, want, bounds, ("dq", "dk", "dv")):
+        _check(a, w, bd, name)
