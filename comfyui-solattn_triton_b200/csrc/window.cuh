@@ -108,7 +108,7 @@ struct WinUnseen {
   int a0, a1, b0;
   __device__ WinUnseen(const WinParams& p, int L, int64_t pa, int64_t pb, int k0, int n) {
     const int hi = win_hi(p, L, pb);
-    a0 = max(0, min(n, p.sinks - k0));
+    a0 = max(0, min(n, min(p.sinks, hi) - k0));   // (sinks past the visible end are not seen either)
     a1 = max(a0, min(n, win_lo(p, pa) - k0));
     b0 = hi < p.Tk ? max(a1, min(n, hi - k0)) : n;   // (past Tk the loads fill in zeros)
   }

@@ -457,3 +457,58 @@ def test_gradient_of_sequences_of_one_key_step(cuda_device, T, H, Hk, D, how):
     _, _, _, _, want, bounds = _definition(*one, dout=do, **how)
     for a, w, bd, name in zip(first, want, bounds, ("dq", "dk", "dv")):
         _check(a, w, bd, name)
+
+
+BELOW_SINKS = [
+    # Tq, Tk, D, how (H 4, Hk 2): fewer visible keys than sinks, by the length or by the right bound
+    (1, 300, 64, dict(left=50, sinks=4, lengths=[1, 3, 2])),
+    (1, 2000, 128, dict(left=200, sinks=1560, lengths=[100, 1, 1501])),
+    (1, 300, 64, dict(sinks=64, lengths=[10, 65, 63])),                      # no left bound
+    (1, 5000, 64, dict(left=4095, sinks=4, lengths=[1, 2, 70])),             # parts of the key axis
+    (20, 2000, 64, dict(left=200, sinks=1560, lengths=[100, 20, 1530])),
+    (150, 700, 128, dict(left=30, sinks=400, lengths=[150, 170, 390])),
+    (40, 300, 64, dict(left=20, sinks=130, offsets=[0, 10, 60])),            # keys that come later
+    (40, 300, 128, dict(left=20, right=5, sinks=70, offsets=[-10, 20, 0])),
+    (333, 333, 64, dict(left=127, sinks=64, lengths=[5, 63, 0], offsets=[0, 0, 0])),
+]
+
+
+@pytest.mark.parametrize("Tq,Tk,D,how", BELOW_SINKS)
+def test_keys_past_the_visible_end_among_the_sinks_are_not_used(cuda_device, Tq, Tk, D, how):
+    """NaN and infinities in every key that no query sees change nothing, also where the visible keys
+    end before the last sink."""
+    q, k, v = (t.cuda() for t in _inputs(3, Tq, Tk, 4, 2, D, seed=Tq + Tk))
+    lengths, offsets = how.get("lengths", [Tk] * 3), how.get("offsets")
+    dev = _device(how)
+    clean = solb200.window_attn(q, k, v, return_lse=True, **dev)
+    dout = torch.randn_like(q)
+    grads = solb200.window_attn_backward(dout, q, k, v, *clean, **dev)
+    k2, v2 = k.clone(), v.clone()
+    for b, n in enumerate(lengths):
+        off = n - Tq if offsets is None else offsets[b]
+        hidden = ~_see(Tq, Tk, n, off, how.get("left"), how.get("right", 0), how["sinks"]).any(0).cuda()
+        assert hidden[:how["sinks"]].any() or n >= how["sinks"]
+        k2[b, hidden], v2[b, hidden] = float("nan"), float("inf")
+    dirty = solb200.window_attn(q, k2, v2, return_lse=True, **dev)
+    assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+    for a, b in zip(grads, solb200.window_attn_backward(dout, q, k2, v2, *dirty, **dev)):
+        assert torch.equal(a, b)
+
+
+def test_streaming_from_the_first_token(cuda_device):
+    """Single tokens into a cache that holds NaN, from the first one on, with more sinks than tokens:
+    as the whole sequence in one call (bound as in test_streaming_layer)."""
+    torch.manual_seed(1)
+    layer = solb200.StreamingSelfAttention(128, 2, head_dim=64, left=6, sinks=16).cuda()
+    layer.qkv.bfloat16()
+    layer.out.bfloat16()
+    x = torch.randn(2, 24, 128, device="cuda").bfloat16()
+    angle = torch.randn(24, 32, device="cuda")
+    with torch.no_grad():
+        whole = layer(x, angle.cos(), angle.sin())
+        cache = layer.new_cache(2, 40)
+        cache.k.fill_(float("nan"))
+        cache.v.fill_(float("nan"))
+        parts = [layer(x[:, t:t + 1], angle[t:t + 1].cos(), angle[t:t + 1].sin(), cache=cache) for t in range(24)]
+    diff = (torch.cat(parts, 1).float() - whole.float()).abs().max().item()
+    assert diff <= 8 * U, diff
