@@ -451,7 +451,9 @@ norm_rope_backward_kernel(const __grid_constant__ RopeParams p, int wdtype) {
       v.load_ring(mine + stage * STAGE + HALF + r * Vec8<T>::PARTS * 512);
       v.get(f);
       to_pairs<INTER>(f, d);
-      const float rs = rsqrtf(fmaf(group_sum2<GL>(a, a), inv_d, p.eps));
+      // (a row that does not exist reads zeros: at eps = 0 its root is infinite, its x^ in the weights' sums NaN)
+      const float root = rsqrtf(fmaf(group_sum2<GL>(a, a), inv_d, p.eps));
+      const float rs = live ? root : 0.f;
       // g: the gradient turned back
       if (INTER) {
 #pragma unroll

@@ -268,3 +268,31 @@ def test_gradient_stays_in_its_workspace(cuda_device, T, H, Hk, D):
     assert rc == 0
     assert (ws[n.value:] == 0xA5).all()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D,R", [(1, 1, 1, 1, 64, 64), (3, 7, 5, 3, 128, 128), (2, 9, 3, 2, 80, 32),
+                                          (1, 37, 9, 3, 256, 256), (1, 64, 8, 8, 64, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_gradient_without_eps(cuda_device, B, T, H, Hk, D, R, dtype, interleaved):
+    """eps = 0, with numbers of rows that do and do not fill the last run: what does not exist adds
+    nothing to the weights' gradients. Bounds as in test_gradient."""
+    q, k, wq, wk, cos, sin = _inputs(B, T, H, Hk, D, R, dtype, seed=10)
+    g = torch.Generator().manual_seed(11)
+    dys = [torch.randn(t.shape, generator=g).to(dtype) for t in (q, k)]
+    args = [t.cuda() for t in (q, k, wq, wk, cos, sin)]
+    outs = solb200.qk_norm_rope(*args, eps=0.0, interleaved=interleaved)
+    got = solb200.qk_norm_rope_backward(*(t.cuda() for t in dys), *args, eps=0.0, interleaved=interleaved)
+    tc, ts = _tables(cos, sin, B)
+    for y, dx, dw, dy, x, w in zip(outs, got[:2], got[2:], dys, (q, k), (wq, wk)):
+        xd, wd = x.double(), w.double()
+        want, r = _formula(xd, wd, tc, ts, interleaved, eps=0.0)
+        _check(y, want, U[dtype] * want.abs() + 24 * 2.0 ** -24 * _partner(xd * r * wd, R, interleaved) + TINY[dtype], "y")
+        gd = _turn(dy.double(), tc, -ts, interleaved)
+        gm = _partner(dy.double(), R, interleaved)
+        xh = xd * r
+        want = r * (gd * wd - xh * (gd * wd * xh).mean(-1, keepdim=True))
+        mags = r * (gm * wd.abs() + xh.abs() * (gm * wd.abs() * xh.abs()).mean(-1, keepdim=True))
+        _check(dx, want, U[dtype] * want.abs() + 32 * 2.0 ** -24 * mags + TINY[dtype], "dx")
+        want = (gd * xh).sum((0, 1, 2))
+        _check(dw, want, U[dtype] * want.abs() + 256 * 2.0 ** -24 * (gm * xh.abs()).sum((0, 1, 2)) + TINY[dtype], "dw")
