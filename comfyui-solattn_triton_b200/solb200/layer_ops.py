@@ -6,9 +6,9 @@ and sliding-window attention with sinks.
                 return_lse=False) -> out or (out, lse)
 
 and their gradients (``qk_norm_rope_backward``, ``window_attn_backward``). The forward calls
-take part in autograd: an input that requires a gradient gets one. Tensors are BTHD as in
-``solb200.ops``; everything runs through libsolb200.so on the current CUDA stream, and there is
-no CPU path. The reference starts at q, k and v that its host has normed and turned, and has
+take part in autograd: an input that requires a gradient gets one (reverse mode; a tangent is
+refused). Tensors are BTHD as in ``solb200.ops``; everything runs through libsolb200.so on the
+current CUDA stream, and there is no CPU path. The reference starts at q, k and v that its host has normed and turned, and has
 no gradient and no windowed attention: these have no counterpart there.
 """
 
@@ -20,6 +20,7 @@ from ctypes import c_float, c_int32, c_int64
 from types import SimpleNamespace
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import I64x2, I64x3, check, lib
 from .ops import _SYNC_CHECK
@@ -89,6 +90,14 @@ def _numbers(**named):
     for name, x in named.items():
         if torch.is_tensor(x):
             _refuse(f"{name} must be a number, not a tensor")
+
+
+def _no_tangents(*tensors):
+    """Refuse forward-mode derivatives: the kernels read values only, a tangent would be dropped."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse("a tensor has a tangent: forward-mode derivatives are not supported")
 
 
 def _fresh(t):
@@ -198,6 +207,7 @@ def _rope_forward(q, k, q_weight, k_weight, cos, sin, eps, interleaved):
 def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, *, eps=1e-6, interleaved=True):
     """(dq, dk, dq_weight, dk_weight) from the gradients of ``qk_norm_rope``'s outputs and its
     inputs. The weights' gradients are summed in fp32 in a fixed order."""
+    _no_tangents(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin)
     plan, q, k, wq, wk, cos, sin = _rope_inputs(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
     for g, x, name in ((dq_out, q, "dq_out"), (dk_out, k, "dk_out")):
         if g.shape != x.shape or g.dtype != x.dtype or g.get_device() != x.get_device():
@@ -241,6 +251,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, eps=1e-6, interleaved=Tr
     or [B, T, R / 2] turn the first R elements of each head, (a, b) -> (a cos - b sin, a sin +
     b cos), on the pairs (2i, 2i + 1) if ``interleaved``, else (i, i + R / 2). D: a multiple of 8
     up to 256, R: of 8 (interleaved) or 16. Weights: the tensors' dtype or float32."""
+    _no_tangents(q, k, q_weight, k_weight, cos, sin)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
                                     or k_weight.requires_grad or cos.requires_grad or sin.requires_grad):
         if cos.requires_grad or sin.requires_grad:
@@ -361,6 +372,7 @@ def window_attn_backward(dout, q, k, v, out, lse, *, left=None, right=0, sinks=0
     """(dq, dk, dv) from the gradient of ``window_attn``'s output, its inputs, its output and
     its log-sum-exp (``return_lse``), with the same bounds. Sums are in a fixed order. ``q`` and
     ``dout`` of queries that see nothing may hold anything (their dq is zero)."""
+    _no_tangents(dout, q, k, v, out, lse)
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
     B, Tq, H, _ = q.shape
     for t, name in ((dout, "dout"), (out, "out")):
@@ -416,6 +428,7 @@ def window_attn(q, k, v, *, left=None, right=0, sinks=0, scale=None, lengths=Non
     anything. Returns a fresh bf16 tensor like q (zeros for a query that sees nothing), and with
     ``return_lse`` also float32 [B, H, Tq], the logarithm of each row's sum (-inf there; it takes
     no gradient)."""
+    _no_tangents(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _WindowAttn.apply(q, k, v, left, right, sinks, scale, lengths, offsets)
     else:

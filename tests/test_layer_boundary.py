@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import solb200
 from solb200 import _lib
@@ -100,3 +101,29 @@ def test_rope_gradient_workspace_holds_every_types_lines(D, lanes):
             if n.value < need * D * 4:
                 short.append((T, H, Hk))
     assert not short
+
+
+def _calls():
+    """The four calls, as (call, its tensors)."""
+    q = torch.randn(1, 8, 2, 64).bfloat16()
+    w, t = torch.ones(64), torch.ones(8, 32)
+    lse = torch.zeros(1, 2, 8)
+    return [(solb200.qk_norm_rope, [q, q, w, w, t, t]), (solb200.qk_norm_rope_backward, [q, q, q, q, w, w, t, t]),
+            (solb200.window_attn, [q, q, q]), (solb200.window_attn_backward, [q, q, q, q, q, lse])]
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be dropped: the calls refuse it, of every tensor; without one they go on
+    to their other checks."""
+    for call, args in _calls():
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                with pytest.raises(RuntimeError, match="CUDA"):
+                    call(*args)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.func.jvp(lambda x: call(*args[:i], x, *args[i + 1:]), (args[i],), (args[i],))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(*args)
