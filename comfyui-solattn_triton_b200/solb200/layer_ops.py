@@ -350,7 +350,8 @@ def _window_forward(q, k, v, left, right, sinks, scale, lengths, offsets, want_l
     plan, q, k, v, lengths, offsets = _window_inputs(q, k, v, left, right, sinks, scale, lengths, offsets)
     B, Tq, H, _ = q.shape
     if plan.empty:      # no queries, or no keys for them to see
-        return (q.new_zeros(q.shape), torch.full((B, H, Tq), -torch.inf, device=q.device) if want_lse else None)
+        lse = torch.full((B, H, Tq), -torch.inf, dtype=torch.float32, device=q.device) if want_lse else None
+        return q.new_zeros(q.shape), lse
     index = q.get_device()
     with _on(index):
         out = _fresh(q)

@@ -512,3 +512,19 @@ def test_streaming_from_the_first_token(cuda_device):
         parts = [layer(x[:, t:t + 1], angle[t:t + 1].cos(), angle[t:t + 1].sin(), cache=cache) for t in range(24)]
     diff = (torch.cat(parts, 1).float() - whole.float()).abs().max().item()
     assert diff <= 8 * U, diff
+
+
+def test_empty_with_another_default_dtype(cuda_device):
+    """The log-sum-exp is float32 whatever torch's default, and the gradient takes it."""
+    q, k, v = (t.cuda() for t in _inputs(2, 5, 7, 4, 2, 64))
+    before = torch.get_default_dtype()
+    try:
+        for dtype in (torch.float64, torch.bfloat16):
+            torch.set_default_dtype(dtype)
+            for kv in ((k[:, :0], v[:, :0]), (k, v)):
+                out, lse = solb200.window_attn(q, *kv, return_lse=True)
+                assert lse.dtype == torch.float32
+                grads = solb200.window_attn_backward(q, q, *kv, out, lse)
+                assert all(t.dtype == torch.bfloat16 for t in grads)
+    finally:
+        torch.set_default_dtype(before)
