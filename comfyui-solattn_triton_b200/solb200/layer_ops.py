@@ -331,18 +331,17 @@ def _device_error(ws, stream, what):
 
 
 # The device error word of calls that need no other workspace, by device and stream: calls of one
-# stream run one after the other, and each clears it first.
+# stream run one after the other, and each clears it first. A captured call takes a word of its
+# own (the graph's memory): its replays may run on another stream beside plain calls.
 _ERROR_WORDS = {}
 
 
 def _workspace(nbytes, q, index, stream):
-    if nbytes > 256:
+    if nbytes > 256 or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     ws = _ERROR_WORDS.get((index, stream))
     if ws is None:
-        ws = torch.empty(256, dtype=torch.uint8, device=q.device)
-        if not torch.cuda.is_current_stream_capturing():     # (a graph's memory is the graph's)
-            _ERROR_WORDS[(index, stream)] = ws
+        ws = _ERROR_WORDS[(index, stream)] = torch.empty(256, dtype=torch.uint8, device=q.device)
     return ws
 
 

@@ -127,3 +127,21 @@ def test_forward_mode_derivatives_are_refused():
                 torch.func.jvp(lambda x: call(*args[:i], x, *args[i + 1:]), (args[i],), (args[i],))
         with pytest.raises(RuntimeError, match="CUDA"):
             call(*args)
+
+
+def test_a_captured_call_has_an_error_word_of_its_own(monkeypatch):
+    """Plain calls of a stream share one word. A graph may be replayed on another stream, beside
+    them: its calls take neither the stream's word nor leave theirs to it."""
+    from solb200 import layer_ops
+    monkeypatch.setattr(layer_ops, "_ERROR_WORDS", {})
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    q = torch.zeros(1)
+    plain = layer_ops._workspace(256, q, 0, 7)
+    assert layer_ops._workspace(256, q, 0, 7) is plain and layer_ops._workspace(256, q, 0, 8) is not plain
+    capturing = True
+    captured = [layer_ops._workspace(256, q, 0, 7) for _ in range(2)] + [layer_ops._workspace(256, q, 0, 9)]
+    assert len({t.data_ptr() for t in (plain, *captured)}) == 4
+    capturing = False
+    assert layer_ops._workspace(256, q, 0, 7) is plain
+    assert all(layer_ops._workspace(256, q, 0, 9) is not t for t in captured)
