@@ -21,21 +21,47 @@ from .layer_ops import qk_norm_rope, window_attn
 
 class KVCache:
     """Keys and values of ``capacity`` tokens per sequence, and how many of them are filled
-    (``lengths``, int32 [B] on the device)."""
+    (``lengths``, int32 [B] on the device; they may be set, or changed in place)."""
 
     def __init__(self, batch, capacity, heads, head_dim, device):
         self.k = torch.empty((batch, capacity, heads, head_dim), dtype=torch.bfloat16, device=device)
         self.v = torch.empty_like(self.k)
-        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):      # (a tensor whose changes are counted in every mode)
+            self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self._rows = torch.arange(batch, device=device)[:, None]
+        self._captured = False                 # replays of a captured call change the lengths uncounted
+        self._at_most(0)
+
+    def _at_most(self, n):
+        """No sequence is longer than n as long as the lengths are this tensor, unchanged."""
+        self._most, self._of = n, self.lengths
+        self._version = None if self.lengths.is_inference() else self.lengths._version
+
+    def _counted(self):
+        return (not self._captured and self._of is self.lengths and self._version is not None
+                and self._version == self.lengths._version)
 
     def append(self, k, v):
-        """Write k / v [B, T, heads, head_dim] behind each sequence's length. The caller keeps the
-        length within the capacity (an index past it is an error of the index operation)."""
-        at = self.lengths[:, None].long() + torch.arange(k.shape[1], device=k.device)
+        """Write k / v [B, T, heads, head_dim] behind each sequence's length; what does not fit the
+        capacity is refused. The lengths are read back for that only where the tokens appended so
+        far could exceed it, or the lengths were changed by someone else. A captured call reads
+        nothing: its tokens past the capacity land on the last place."""
+        T, capacity = k.shape[1], self.k.shape[1]
+        capturing = self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+        self._captured = self._captured or capturing
+        if self.lengths.numel() and T and not capturing:
+            if not self._counted() or self._most + T > capacity:
+                self._at_most(int(self.lengths.max()))
+            if self._most + T > capacity:
+                raise RuntimeError(f"solb200: {T} tokens behind {self._most} do not fit a cache of {capacity}")
+        elif T > capacity:
+            raise RuntimeError(f"solb200: {T} tokens do not fit a cache of {capacity}")
+        # (an index outside the cache would be a device assertion)
+        at = (self.lengths[:, None] + torch.arange(T, device=k.device)).clamp_(0, capacity - 1)
         self.k[self._rows, at] = k
         self.v[self._rows, at] = v
-        self.lengths += k.shape[1]
+        self.lengths += T
+        self._at_most(self._most + T)
 
 
 class StreamingSelfAttention(torch.nn.Module):
