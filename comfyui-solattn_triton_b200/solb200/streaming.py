@@ -9,7 +9,8 @@ the first tokens kept visible (``window_attn``), projection.
 
 A chunk's tokens see the chunk, the window before it and the sinks. With ``cache`` the new keys
 and values are written behind each sequence's length, which stays on the device: a step makes no
-host copy. ``lengths`` of ragged sequences (right-padded) may be set on the cache.
+host copy. ``lengths`` of ragged sequences (right-padded) may be set on the cache. A call with a
+cache is inference: it records nothing for a gradient, and refuses an input that requires one.
 """
 
 from __future__ import annotations
@@ -45,7 +46,8 @@ class KVCache:
         """Write k / v [B, T, heads, head_dim] behind each sequence's length; what does not fit the
         capacity is refused. The lengths are read back for that only where the tokens appended so
         far could exceed it, or the lengths were changed by someone else. A captured call reads
-        nothing: its tokens past the capacity land on the last place."""
+        nothing: its tokens past the capacity land on the last place. The cache takes the values
+        alone: no gradient goes through it."""
         T, capacity = k.shape[1], self.k.shape[1]
         capturing = self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
         self._captured = self._captured or capturing
@@ -58,8 +60,8 @@ class KVCache:
             raise RuntimeError(f"solb200: {T} tokens do not fit a cache of {capacity}")
         # (an index outside the cache would be a device assertion)
         at = (self.lengths[:, None] + torch.arange(T, device=k.device)).clamp_(0, capacity - 1)
-        self.k[self._rows, at] = k
-        self.v[self._rows, at] = v
+        self.k[self._rows, at] = k.detach()
+        self.v[self._rows, at] = v.detach()
         self.lengths += T
         self._at_most(self._most + T)
 
@@ -83,6 +85,12 @@ class StreamingSelfAttention(torch.nn.Module):
         return KVCache(batch, capacity, self.kv_heads, self.head_dim, self.qkv.weight.device)
 
     def forward(self, x, cos, sin, cache=None):
+        if cache is not None and torch.is_grad_enabled():
+            if x.requires_grad:
+                raise RuntimeError("solb200: a call with a cache takes no gradient, and its input requires one; "
+                                   "make it under torch.no_grad()")
+            with torch.no_grad():
+                return self.forward(x, cos, sin, cache)
         B, T, _ = x.shape
         qkv = self.qkv(x).view(B, T, -1, self.head_dim)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=2)

@@ -81,6 +81,22 @@ def test_no_sequences_and_no_tokens():
     assert cache.lengths.tolist() == [2, 2]
 
 
+def test_the_cache_keeps_values_not_their_history():
+    cache = solb200.KVCache(1, 4, 1, 2, "cpu")
+    k = _tokens(1, 2, 0).requires_grad_()
+    cache.append(k * 2, k * 3)
+    assert not cache.k.requires_grad and not cache.v.requires_grad
+    assert cache.k[0, :2, 0, 0].tolist() == [0, 2] and cache.v[0, :2, 0, 0].tolist() == [0, 3]
+
+
+def test_a_cached_call_refuses_an_input_that_requires_a_gradient():
+    layer = solb200.StreamingSelfAttention(16, 1, head_dim=64)
+    cache = layer.new_cache(1, 4)
+    with pytest.raises(RuntimeError, match="solb200.*gradient"):
+        layer(torch.zeros(1, 1, 16, requires_grad=True), torch.zeros(1, 32), torch.zeros(1, 32), cache=cache)
+    assert cache.lengths.tolist() == [0]
+
+
 @pytest.mark.gpu
 def test_a_captured_step_past_the_capacity_stays_in_the_cache(cuda_device):
     """Replays read nothing back: past the capacity the last place takes the token, nothing outside
@@ -104,3 +120,24 @@ def test_a_captured_step_past_the_capacity_stays_in_the_cache(cuda_device):
     cache.lengths.fill_(3)
     cache.append(token, token)
     assert cache.lengths.tolist() == [4, 4] and cache.k[0, 3, 0, 0] == 9
+
+
+@pytest.mark.gpu
+def test_cached_calls_with_gradients_enabled_keep_no_graph(cuda_device):
+    """The layer's parameters require gradients: a stream without no_grad() gives the same values and
+    leaves neither the cache nor the output with a history."""
+    torch.manual_seed(2)
+    layer = solb200.StreamingSelfAttention(128, 2, head_dim=64, left=6, sinks=2).cuda()
+    layer.qkv.bfloat16()
+    layer.out.bfloat16()
+    x = torch.randn(2, 5, 128, device="cuda").bfloat16()
+    angle = torch.randn(5, 32, device="cuda")
+    runs = []
+    for enabled in (True, False):
+        with torch.set_grad_enabled(enabled):
+            cache = layer.new_cache(2, 8)
+            cache.k.zero_()
+            runs.append([layer(x[:, t:t + 1], angle[t:t + 1].cos(), angle[t:t + 1].sin(), cache=cache) for t in range(5)])
+            assert not cache.k.requires_grad and not cache.v.requires_grad
+    for a, b in zip(*runs):
+        assert torch.equal(a, b) and not a.requires_grad
