@@ -43,12 +43,16 @@ __device__ __forceinline__ int64_t order_row(const int64_t* perm, int64_t r, int
 }
 
 // Programmatic dependent launch. Every kernel of the path is launched with
-// programmaticStreamSerializationAllowed (launch_pdl), and its first statement is
-// pdl_begin(): griddepcontrol.wait returns once the preceding grid in the stream has
+// programmaticStreamSerializationAllowed (launch_pdl) and calls pdl_begin() before it touches
+// global memory: griddepcontrol.wait returns once the preceding grid in the stream has
 // completed and its memory is visible (at once when there is no such grid), then
 // griddepcontrol.launch_dependents lets the next kernel's CTAs be scheduled while this
-// one runs; they in turn wait in their own pdl_begin(). Nothing is read or written
-// before the wait, so the overlap is the next launch's setup and CTA placement only.
+// one runs; they in turn wait in their own pdl_begin(). No global memory is read or written
+// before the wait, so the overlap is the next launch's setup and CTA placement only. Most kernels
+// call it first; the windowed attention kernels before it prefetch tensor maps, set up barriers and
+// take tensor memory. What they hold while they wait is not missing to the grid they wait for: a
+// kernel of the path takes 256 columns with about 100 KB of shared memory, or all 512 with more than
+// half of an SM's, so the CTAs that fit an SM together never want more than it has.
 __device__ __forceinline__ void pdl_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

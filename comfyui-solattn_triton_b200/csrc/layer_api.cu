@@ -95,7 +95,7 @@ constexpr int kStepKeys = 64, kTileRows = 128;
 // lengths live on the device) but together no shorter than the GPU needs at nine tenths of its slots,
 // and kOpen steps to open and close each; the joining kernel takes kJoin and reads what the parts
 // wrote (`row_bytes` each, there and back at 5 MB a step), a third of a step per part.
-// Measured (us): 8 tiles x 64 steps 53 whole, 17.6 in 9 parts, 26.9 in 60; 40 tiles x 4096
+// Measured (us, short bursts): 8 tiles x 64 steps 53 whole, 17.6 in 9 parts, 26.9 in 60; 40 tiles x 4096
 // steps 2841 whole, 755 in 7, 946 in 9 (two waves), 784 in 22; 520 tiles x 195 steps 451 whole, 479 in 2.
 int window_splits(int64_t tiles, int64_t steps, int64_t row_bytes) {
   constexpr double kOpen = 3, kJoin = 2;
@@ -118,7 +118,7 @@ int window_splits(int64_t tiles, int64_t steps, int64_t row_bytes) {
 
 // The gradient's parts, in steps of one CTA (about 2 us each, one CTA per SM): `most` steps of the longest
 // tile, `mean` of all of them, kOpen to open and close a CTA; the joining kernel takes kJoin and moves
-// part_bytes per part there and back (8 MB a step). Measured, forward and gradient (us): 2 heads x 2000
+// part_bytes per part there and back (8 MB a step). Measured in short bursts, forward and gradient (us): 2 heads x 2000
 // causal tokens 84 whole, 65 in parts; 2 x 4000 in a window of 200 with 64 sinks 102 and 69; 8 x 800 53 and 59.
 int gradient_splits(int64_t tiles, int64_t most, double mean, int64_t part_bytes) {
   constexpr double kOpen = 3, kJoin = 3.5, kSms = 148;

@@ -29,8 +29,8 @@ namespace solb200 {
 namespace {
 
 constexpr int kRopeThreads = 256;
-// Rows per lane group of a run, and runs a warp has in flight or at work. Measured (bf16; forward
-// 32760 x 80 rows of 128, backward 16384 x 48): forward 4 rows x 3 runs 212 us (6.3 TB/s), x 2
+// Rows per lane group of a run, and runs a warp has in flight or at work. Measured (bf16, short
+// bursts; back to back 221 - 229 and 107 - 113 us; forward 32760 x 80 rows of 128, backward 16384 x 48): forward 4 rows x 3 runs 212 us (6.3 TB/s), x 2
 // 252 us, x 4 229 us, 2 rows with a register prefetch 255 us; backward 4 rows x 2 runs 108 us
 // (weights' join included; 5.6 TB/s), 2 rows x 3 runs 120 us. Three CTAs an SM: 64 registers for four
 // spill (260 and 152 us).

@@ -16,8 +16,8 @@
 // columns; 256 threads took 616 us where these took 566, in the first form of window_dkv_kernel), one
 // TMA warp, one MMA warp, one CTA per SM.
 //
-// Measured on a B200, 4 x 4096 tokens x 24 heads x 128, about 1000 keys a row: window_dq_kernel 370 us,
-// window_dkv_kernel 472 us, 0.90 and 0.94 PFLOP/s of products executed. An iteration takes 2400 and
+// Measured on a B200, 4 x 4096 tokens x 24 heads x 128, about 1000 keys a row, in short bursts: window_dq_kernel
+// 370 us, window_dkv_kernel 472 us, 0.90 and 0.94 PFLOP/s of products executed. An iteration takes 2400 and
 // 3300 cycles against 1536 and 2048 of products: the softmax threads are busy for most of them, and
 // only what the barriers allow runs at the same time.
 //

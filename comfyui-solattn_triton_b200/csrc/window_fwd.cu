@@ -19,9 +19,11 @@
 //
 // Keys that no row of the tile sees may hold anything (WinUnseen).
 //
-// Measured on a B200, 40 heads x 128: 32760 queries seeing about 5940 keys each 3.5 ms (1.14 PFLOP/s; 4.07 ms
-// and 0.98 at the power cap), bound by one CTA's softmax and the other's products taking turns
-// (tensor pipe 59 % busy, exponentials 60 %); one token over 262001 keys 755 us (7.1 TB/s).
+// Measured on a B200, 40 heads x 128: 32760 queries seeing about 5940 keys each 3.5 ms in a short
+// burst (1.14 PFLOP/s), 4.0 back to back (0.99, at the power cap), bound by one CTA's softmax and the
+// other's products taking turns (tensor pipe 59 % busy, exponentials 60 %); one token over 262001 keys
+// 744 us in a burst (7.2 TB/s, reads alone), 796 - 858 back to back (6.7 - 6.3; a copy, which writes
+// too, runs at 6.56).
 #include "fwd_common.cuh"
 #include "window.cuh"
 
